@@ -13,6 +13,7 @@ fp = C.c_void_p          # device pointers travel as integers
 i32 = C.c_int
 f32 = C.c_float
 sz = C.c_size_t
+i64 = C.c_longlong
 
 
 class LstmDir(C.Structure):
@@ -70,6 +71,16 @@ class HyperScanDesc(C.Structure):
                 ('dir', HyperDir * 2)]
 
 
+class SscanDesc(C.Structure):
+    _fields_ = [(n, i32) for n in ('T', 'B', 'D', 'N', 'G', 'dtype', 'reverse', 'softplus')] + [
+        ('lens', fp), ('x', fp), ('x_st', i64), ('x_sb', i64), ('dt', fp), ('dt_st', i64), ('dt_sb', i64),
+        ('z', fp), ('z_st', i64), ('z_sb', i64), ('Bm', fp), ('b_st', i64), ('b_sb', i64), ('b_sg', i64),
+        ('Cm', fp), ('c_st', i64), ('c_sb', i64), ('c_sg', i64), ('A', fp), ('Dk', fp), ('dt_bias', fp), ('h0', fp),
+        ('out', fp), ('o_st', i64), ('o_sb', i64), ('h_last', fp), ('ckpt', fp),
+        ('dout', fp), ('do_st', i64), ('do_sb', i64), ('dh_last', fp)] + [
+        (n, fp) for n in ('dx', 'ddt', 'dz', 'dB', 'dC', 'dA', 'dD', 'ddt_bias', 'dh0')]
+
+
 _SIGS = {
     'asr_gemm_f32': (i32, [i32, i32, i32, i32, i32, f32, fp, i32, fp, i32, f32, fp, i32, fp, fp]),
     'asr_gemm_f32_ws': (i32, [i32, i32, i32, i32, i32, f32, fp, i32, fp, i32, f32, fp, i32, fp, fp, sz, fp]),
@@ -124,6 +135,22 @@ _SIGS = {
     'asr_hyper_scan_ws_bytes': (sz, [i32, i32, i32, i32, i32, i32]),
     'asr_hyper_scan_fwd': (i32, [C.POINTER(HyperScanDesc), fp, sz, fp]),
     'asr_hyper_scan_bwd': (i32, [C.POINTER(HyperScanDesc), fp, sz, fp]),
+    'asr_conv_fwd': (i32, [i32, i32, i32, i32, i32, fp, i64, i64, fp, fp, fp, fp, i32, i32, fp, i64, i64, fp, fp]),
+    'asr_conv_bwd_ws_bytes': (sz, [i32, i32, i32, i32]),
+    'asr_conv_bwd': (i32, [i32, i32, i32, i32, i32, fp, i64, i64, fp, i64, i64, fp, fp, fp, fp, i32, i32, fp, fp, fp, fp, fp,
+                           sz, fp]),
+    'asr_conv_step': (i32, [i32, i32, i32, i32, fp, i64, fp, fp, fp, i32, fp, i64, fp]),
+    'asr_sscan_ckpt_floats': (sz, [i32, i32, i32, i32]),
+    'asr_sscan_ws_bytes': (sz, [i32, i32, i32, i32, i32, i32]),
+    'asr_sscan_fwd': (i32, [C.POINTER(SscanDesc), fp, sz, fp]),
+    'asr_sscan_bwd': (i32, [C.POINTER(SscanDesc), fp, sz, fp]),
+    'asr_sscan_step': (i32, [i32, i32, i32, i32, i32, fp, fp, i64, fp, i64, fp, fp, i64, i64, fp, i64, i64, fp, fp, i64, fp,
+                             i32, fp, i64, fp]),
+    'asr_rms_norm_fwd': (i32, [i32, fp, i64, fp, i64, fp, i32, i32, f32, fp, fp, fp, fp]),
+    'asr_rms_norm_bwd_ws_bytes': (sz, [i32, i32]),
+    'asr_rms_norm_bwd': (i32, [i32, fp, i64, fp, i64, fp, i64, fp, fp, fp, i64, i32, i32, fp, fp, fp, sz, fp]),
+    'asr_clip_list_ws_bytes': (sz, [i32, C.POINTER(i64)]),
+    'asr_clip_list': (i32, [i32, C.POINTER(i32), C.POINTER(fp), C.POINTER(fp), C.POINTER(i64), f32, f32, fp, fp, sz, fp]),
 }
 
 _lib = None

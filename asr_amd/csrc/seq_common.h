@@ -1,0 +1,82 @@
+// Shared by the state-space layer's kernels (conv.hip, sscan_*.hip, rmsnorm.hip): activation types and lane sums.
+#pragma once
+#include "common.h"
+
+#define ASR_F32 0
+#define ASR_BF16 1
+#define ASR_F16 2
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// Activations are held in f32, bf16 or f16 and computed in f32; a store rounds once, to nearest even.
+template <typename T> __device__ __forceinline__ float ldf(const T* p) { return (float)*p; }
+template <typename T> __device__ __forceinline__ void stf(T* p, float v) { *p = (T)v; }
+
+// V consecutive values as one access (V * sizeof(T) = 16 bytes, or V = 1)
+template <typename T, int V> struct Vec { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T> struct Vec<T, 1> { typedef T type; };
+template <typename T, int V> __device__ __forceinline__ void ldv(const T* p, float* o) {
+    if constexpr (V == 1) o[0] = (float)p[0];
+    else {
+        const typename Vec<T, V>::type v = *(const typename Vec<T, V>::type*)p;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = (float)v[e];
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void stv(T* p, const float* o) {
+    if constexpr (V == 1) p[0] = (T)o[0];
+    else {
+        typename Vec<T, V>::type v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = (T)o[e];
+        *(typename Vec<T, V>::type*)p = v;
+    }
+}
+
+__device__ __forceinline__ float silu_(float z) { return z * sigmoidf_(z); }
+// d silu / dz, from z and its sigmoid
+__device__ __forceinline__ float dsilu_(float z, float sg) { return sg * (1.0f + z * (1.0f - sg)); }
+// log(1 + e^v) without overflow and with relative accuracy for very negative v
+__device__ __forceinline__ float softplus_(float v) { return fmaxf(v, 0.0f) + log1pf(expf_(-fabsf(v))); }
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// a frame of row b: walking order s -> frame.  Both directions walk the valid frames s = 0 .. len-1.
+__device__ __forceinline__ int row_len(const int* lens, int b, int T) {
+    if (!lens) return T;
+    const int n = lens[b];
+    return n < 0 ? 0 : (n > T ? T : n);
+}
+
+// out[i] = sum over p of part[p * stride + i], i < n, in a fixed order: the second half of every reduction over rows or
+// time.  64 columns x 16 groups of partials per workgroup; a group adds its partials in order, the groups are joined in
+// order in LDS.
+static __global__ __launch_bounds__(1024) void sum_partials_kernel(const float* __restrict__ part, size_t stride, int P,
+                                                                   size_t n, float* __restrict__ out) {
+    __shared__ float sm[16][65];
+    const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const size_t i = (size_t)blockIdx.x * 64 + c;
+    float acc = 0.f;
+    if (i < n)
+        for (int p = g; p < P; p += 16) acc += part[(size_t)p * stride + i];
+    sm[g][c] = acc;
+    __syncthreads();
+    if (g == 0 && i < n) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t += sm[k][c];
+        out[i] = t;
+    }
+}
+static inline void sum_partials(const float* part, size_t stride, int P, size_t n, float* out, hipStream_t stream) {
+    if (n) hipLaunchKernelGGL(sum_partials_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, stream, part, stride, P,
+                              n, out);
+}
+
+static inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+static inline size_t elem_size(int dtype) { return dtype == ASR_F32 ? 4 : 2; }

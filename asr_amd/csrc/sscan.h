@@ -1,0 +1,69 @@
+// Selective state-space scan: what its forward and backward kernels share.
+//   delta = softplus(dt + dt_bias)  (or dt + dt_bias),   a = exp(delta A)
+//   h[s] = a h[s-1] + (delta x) B[s],   y = sum_n C[s] h[s] + D x,   out = y silu(z)  (or y)
+// per row b, channel d and state n; B and C are shared by the channels of a group.
+//
+// A workgroup is 64 channels (one per lane, so every activation row is one coalesced access) times all states: each of its
+// four waves holds SPL states per channel in registers (NB times over for more than 16 states) and walks TS frames per tile.
+// What does not depend on the state (delta, delta x, gates) is formed once per (frame, channel) by the four waves together
+// and handed over in LDS, B and C as broadcast reads.
+#pragma once
+#include "seq_common.h"
+#include "../../include/asr_amd.h"      // asr_sscan_desc
+
+#define SSCAN_TS 16          // frames of a tile; the training forward pass saves the state in front of every tile
+
+struct SscanArgs {
+    int T, B, D, N, G, dpg, tpg;     // dpg: channels of a group, tpg: 64-channel tiles of a group
+    int reverse, softplus;
+    int S, tpc;                      // time is cut into S chunks of tpc tiles each
+    int np;                          // states, padded to what the waves hold
+    int vec;                         // single frames: the state and A can be read 16 bytes at a time
+    const int* lens;
+    const void *x, *dt, *z, *Bm, *Cm;
+    long long x_st, x_sb, dt_st, dt_sb, z_st, z_sb, b_st, b_sb, b_sg, c_st, c_sb, c_sg;
+    const float *A, *Dk, *bias, *h0;
+    void* out; long long o_st, o_sb;
+    float *h_last, *ckpt;
+    const void* dout; long long do_st, do_sb;
+    const float* dh_last;
+    void *dx, *ddt, *dz;
+    float* dh0;
+    float *c_h, *c_ds;               // per chunk: its own final state (or first adjoint), its sum of delta
+    float *part_bc, *part_a, *part_d, *part_b;
+};
+
+#define LOG2E 1.4426950408889634f
+#define LN2 0.6931471805599453f
+
+// states a wave holds per channel (SPL) and how often (NB): 4 waves * SPL * NB >= N
+static inline int sscan_spl(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }
+static inline int sscan_nb(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
+static inline int sscan_np(int N) { return 4 * sscan_spl(N) * sscan_nb(N); }
+static inline int sscan_tiles(int T) { return (T + SSCAN_TS - 1) / SSCAN_TS; }
+
+int sscan_chunks(int T, int B, int D, int N, int G, int backward);
+int sscan_fill(const asr_sscan_desc* d, SscanArgs* p, int backward);
+
+// What a thread of the workgroup knows about its place.
+struct Place {
+    int lane, w, b, g, ct, d, len, nt, t0, t1, k;
+    bool on;
+};
+__device__ __forceinline__ Place sscan_place(const SscanArgs& p) {
+    Place q;
+    q.lane = threadIdx.x & 63;
+    q.w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    q.g = blockIdx.x / p.tpg;
+    q.ct = blockIdx.x % p.tpg;
+    q.b = blockIdx.y;
+    q.k = blockIdx.z;
+    const int dl = q.ct * 64 + q.lane;
+    q.on = dl < p.dpg;
+    q.d = q.g * p.dpg + (q.on ? dl : p.dpg - 1);
+    q.len = row_len(p.lens, q.b, p.T);
+    q.nt = (q.len + SSCAN_TS - 1) / SSCAN_TS;          // tiles that hold a valid frame
+    q.t0 = q.k * p.tpc;
+    q.t1 = min(q.t0 + p.tpc, q.nt);                     // this chunk's tiles; none if t1 <= t0
+    return q;
+}

@@ -1,0 +1,340 @@
+// Backward pass of the selective scan.  With q = dh a h[s-1]:
+//   dh[s] = C dy + a[s+1] dh[s+1],   dC = sum_d dy h,   dB = sum_d dh delta x,
+//   dA = sum_s delta q,   d delta = sum_n A q + x sum_n dh B,   dx = delta sum_n dh B + D dy,   dz = dout y silu'(z)
+// Tiles are walked from the last to the first.  A tile's states are formed again from the state saved in front of it and kept
+// in registers (16 frames x states, with a), then the adjoint runs back over them.
+#include "sscan.h"
+
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float half_join(float a, float b) {      // lanes 0-31: a[l] + a[l+32], lanes 32-63: the same of b
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+__device__ __forceinline__ float row_join(float a, float b) {       // even 16-lane rows: a's pair of rows, odd: b's
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+// Sums over the 64 lanes of sixteen values at once: lane l returns the sum of v[l >> 2].  Each of the first four steps joins
+// two values in one register and halves the lanes that still have to be added: 35 instructions for 16 sums (96 one by one).
+__device__ __forceinline__ float sum16(const float (&v)[16], int lane) {
+    float w[8], x[4], y[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = half_join(v[i], v[i + 8]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = row_join(w[i], w[i + 4]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float keep = (lane & 8) ? x[i + 2] : x[i], give = (lane & 8) ? x[i] : x[i + 2];
+        y[i] = keep + dpp<0x128>(give);                              // row_ror:8
+    }
+    const float keep = (lane & 4) ? y[1] : y[0], give = (lane & 4) ? y[0] : y[1];
+    float z = keep + dpp<0x141>(give);                               // row_half_mirror
+    z += dpp<0xB1>(z);                                               // quad_perm [1,0,3,2]
+    return z + dpp<0x4E>(z);                                         // quad_perm [2,3,0,1]
+}
+
+// PRE: the adjoint a chunk hands to the one in front of it when nothing comes in from behind, and its sum of delta.
+template <typename TY, int SPL, int NB, bool PRE>
+__global__ __launch_bounds__(256) void sstate_bwd_kernel(SscanArgs p) {
+    constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RS = 8 / SPL;    // RS frames give sixteen sums
+    __shared__ float2 s_du[TS][64];
+    __shared__ float s_dy[TS][64];
+    __shared__ __attribute__((aligned(16))) float s_B[PRE ? 1 : TS][NP], s_C[TS][NP];
+    __shared__ float2 s_s[PRE ? 1 : 4][PRE ? 1 : TS][64];
+    __shared__ float s_y[PRE ? 1 : 4][PRE ? 1 : TS][64];
+    __shared__ float s_bc[PRE ? 1 : TS][2][NP];
+    const Place q = sscan_place(p);
+    const int tid = threadIdx.x, lane = q.lane, w = q.w;
+    if (PRE && (q.k == 0 || q.t0 >= q.t1)) return;
+    const TY* px = (const TY*)p.x + q.b * p.x_sb + q.d;
+    const TY* pdt = (const TY*)p.dt + q.b * p.dt_sb + q.d;
+    const TY* pz = p.z ? (const TY*)p.z + q.b * p.z_sb + q.d : nullptr;
+    const TY* pdo = (const TY*)p.dout + q.b * p.do_sb + q.d;
+    const TY* pB = (const TY*)p.Bm + q.b * p.b_sb + q.g * p.b_sg;
+    const TY* pC = (const TY*)p.Cm + q.b * p.c_sb + q.g * p.c_sg;
+    const size_t obase = (size_t)q.b * p.D + q.d, ostep = (size_t)p.B * p.D;
+    const float bias = p.bias ? p.bias[q.d] : 0.f;
+    const float Dk = p.Dk ? p.Dk[q.d] : 0.f;
+    float A2[NB][SPL], r[NB][SPL], dA[NB][SPL];
+#pragma unroll
+    for (int m = 0; m < NB; ++m)
+#pragma unroll
+        for (int j = 0; j < SPL; ++j) {
+            const int n = (m * 4 + w) * SPL + j;
+            A2[m][j] = n < p.N ? p.A[(size_t)q.d * p.N + n] * LOG2E : 0.f;
+            r[m][j] = (!PRE && p.dh_last && n < p.N) ? p.dh_last[((size_t)q.b * p.D + q.d) * p.N + n] : 0.f;
+            dA[m][j] = 0.f;
+        }
+    const int nch = (q.nt + p.tpc - 1) / p.tpc;                       // chunks that hold a valid frame
+    if (!PRE) {                                                       // the adjoint that comes in from behind
+        for (int j = nch - 1; j > q.k; --j) {
+            const float ds = p.c_ds[((size_t)j * p.B + q.b) * p.D + q.d];
+#pragma unroll
+            for (int m = 0; m < NB; ++m)
+#pragma unroll
+                for (int i = 0; i < SPL; ++i) {
+                    const int n = (m * 4 + w) * SPL + i;
+                    const float rl = p.c_h[(((size_t)j * p.B + q.b) * NP + n) * p.D + q.d];
+                    r[m][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][i] * ds), r[m][i], rl);
+                }
+        }
+    }
+    if (!q.on) {                                // idle lanes stand on a real channel: they must give nothing to dB and dC
+#pragma unroll
+        for (int m = 0; m < NB; ++m)
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) r[m][j] = 0.f;
+    }
+    float accD = 0.f, accb = 0.f, dsum = 0.f;
+    for (int tile = q.t1 - 1; tile >= q.t0; --tile) {
+        const int sb = tile * TS;
+        float rx[4], rz[4], rg[4], rr[4], rd[4], ry[4];              // own frames: x, z, dout, dt + bias, delta, dy
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = sb + w * 4 + i;
+            rx[i] = rz[i] = rg[i] = rr[i] = rd[i] = ry[i] = 0.f;
+            if (s < q.len) {
+                const long long f = p.reverse ? q.len - 1 - s : s;
+                rx[i] = ldf(px + f * p.x_st);
+                rr[i] = ldf(pdt + f * p.dt_st) + bias;
+                rg[i] = ldf(pdo + f * p.do_st);
+                if (pz) rz[i] = ldf(pz + f * p.z_st);
+                rd[i] = p.softplus ? softplus_(rr[i]) : rr[i];
+                ry[i] = pz ? rg[i] * silu_(rz[i]) : rg[i];
+            }
+            s_du[w * 4 + i][lane] = float2{rd[i], q.on ? rd[i] * rx[i] : 0.f};
+            s_dy[w * 4 + i][lane] = q.on ? ry[i] : 0.f;
+        }
+        for (int i = tid; i < TS * NP; i += 256) {
+            const int st = i / NP, n = i % NP, s = sb + st;
+            float vb = 0.f, vc = 0.f;
+            if (s < q.len && n < p.N) {
+                const long long f = p.reverse ? q.len - 1 - s : s;
+                if (!PRE) vb = ldf(pB + f * p.b_st + n);
+                vc = ldf(pC + f * p.c_st + n);
+            }
+            if (!PRE) s_B[st][n] = vb;
+            s_C[st][n] = vc;
+        }
+        __syncthreads();
+        if (PRE) {
+#pragma unroll 4
+            for (int t = TS - 1; t >= 0; --t) {
+                const float de = s_du[t][lane].x, dy = s_dy[t][lane];
+#pragma unroll
+                for (int m = 0; m < NB; ++m)
+#pragma unroll
+                    for (int j = 0; j < SPL; ++j)
+                        r[m][j] = __builtin_amdgcn_exp2f(A2[m][j] * de) * __builtin_fmaf(s_C[t][(m * 4 + w) * SPL + j], dy, r[m][j]);
+                if (w == 0) dsum += de;
+            }
+            __syncthreads();
+            continue;
+        }
+        const float* ck = p.ckpt + ((size_t)tile * p.B + q.b) * NP * p.D + q.d;
+#pragma unroll
+        for (int m = 0; m < NB; ++m) {
+            float a[TS][SPL], h[TS][SPL], h0[SPL], da[SPL];    // da: a tile's part of dA, so that no sum runs over all frames
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) da[j] = 0.f;
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) h0[j] = ck[(size_t)((m * 4 + w) * SPL + j) * p.D];
+#pragma unroll
+            for (int t = 0; t < TS; ++t) {
+                const float2 du = s_du[t][lane];
+                float y = 0.f;
+#pragma unroll
+                for (int j = 0; j < SPL; ++j) {
+                    const int n = (m * 4 + w) * SPL + j;
+                    a[t][j] = __builtin_amdgcn_exp2f(A2[m][j] * du.x);
+                    h[t][j] = __builtin_fmaf(a[t][j], t ? h[t - 1][j] : h0[j], du.y * s_B[t][n]);
+                    y = __builtin_fmaf(s_C[t][n], h[t][j], y);
+                }
+                if (pz) { if (m) s_y[w][t][lane] += y; else s_y[w][t][lane] = y; }
+            }
+#pragma unroll
+            for (int tb = TS / RS - 1; tb >= 0; --tb) {
+                float v[16];
+#pragma unroll
+                for (int i = RS - 1; i >= 0; --i) {
+                    const int t = tb * RS + i;
+                    const float2 du = s_du[t][lane];
+                    const float dy = s_dy[t][lane];
+                    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+                    for (int j = 0; j < SPL; ++j) {
+                        const int n = (m * 4 + w) * SPL + j;
+                        const float dh = __builtin_fmaf(s_C[t][n], dy, r[m][j]);
+                        v[i * 2 * SPL + j] = dh * du.y;
+                        v[i * 2 * SPL + SPL + j] = dy * h[t][j];
+                        r[m][j] = a[t][j] * dh;
+                        const float qq = r[m][j] * (t ? h[t - 1][j] : h0[j]);
+                        s2 = __builtin_fmaf(qq, A2[m][j], s2);
+                        da[j] = __builtin_fmaf(qq, du.x, da[j]);
+                        s1 = __builtin_fmaf(dh, s_B[t][n], s1);
+                    }
+                    if (m) { s_s[w][t][lane].x += s1; s_s[w][t][lane].y += s2; }
+                    else s_s[w][t][lane] = float2{s1, s2};
+                }
+                const float z = sum16(v, lane);
+                if ((lane & 3) == 0) {
+                    const int id = lane >> 2, t = tb * RS + id / (2 * SPL), c = (id / SPL) & 1, j = id % SPL;
+                    s_bc[t][c][(m * 4 + w) * SPL + j] = z;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) dA[m][j] += da[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = w * 4 + i, s = sb + t;
+            if (s >= p.T || !q.on) continue;
+            const float s1 = (s_s[0][t][lane].x + s_s[1][t][lane].x) + (s_s[2][t][lane].x + s_s[3][t][lane].x);
+            const float s2 = (s_s[0][t][lane].y + s_s[1][t][lane].y) + (s_s[2][t][lane].y + s_s[3][t][lane].y);
+            const bool ok = s < q.len;
+            const long long f = (p.reverse && ok) ? q.len - 1 - s : s;
+            const size_t o = f * ostep + obase;
+            float ddt = __builtin_fmaf(rx[i], s1, s2 * LN2);
+            if (p.softplus) ddt *= sigmoidf_(rr[i]);
+            stf((TY*)p.dx + o, ok ? __builtin_fmaf(rd[i], s1, Dk * ry[i]) : 0.f);
+            stf((TY*)p.ddt + o, ok ? ddt : 0.f);
+            if (pz) {
+                const float y = ((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i];
+                stf((TY*)p.dz + o, ok ? rg[i] * y * dsilu_(rz[i], sigmoidf_(rz[i])) : 0.f);
+            }
+            if (ok) { accD = __builtin_fmaf(ry[i], rx[i], accD); accb += ddt; }
+        }
+        float* pbc = p.part_bc + (((size_t)(q.g * p.tpg + q.ct) * p.B + q.b) * p.T + sb) * (2 * NP);
+        for (int i = tid; i < TS * 2 * NP; i += 256)
+            if (sb + i / (2 * NP) < q.len) pbc[i] = s_bc[i / (2 * NP)][(i / NP) & 1][i % NP];
+        __syncthreads();
+    }
+    if (PRE) {
+        if (!q.on) return;
+#pragma unroll
+        for (int m = 0; m < NB; ++m)
+#pragma unroll
+            for (int j = 0; j < SPL; ++j)
+                p.c_h[(((size_t)q.k * p.B + q.b) * NP + (m * 4 + w) * SPL + j) * p.D + q.d] = r[m][j];
+        if (w == 0) p.c_ds[((size_t)q.k * p.B + q.b) * p.D + q.d] = dsum;
+        return;
+    }
+    // padding, the parts of the parameter gradients, the gradient of the first state
+    const int send = min(p.T, (q.t0 + p.tpc) * TS);
+    if (q.on) {
+        for (int s = max(q.nt, q.t0) * TS + w; s < send; s += 4) {
+            const size_t o = s * ostep + obase;
+            stf((TY*)p.dx + o, 0.f);
+            stf((TY*)p.ddt + o, 0.f);
+            if (pz) stf((TY*)p.dz + o, 0.f);
+        }
+    }
+    const size_t row = (size_t)q.k * p.B + q.b;
+    if (q.on) {
+#pragma unroll
+        for (int m = 0; m < NB; ++m)
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) {
+                const int n = (m * 4 + w) * SPL + j;
+                if (n >= p.N) continue;
+                p.part_a[(row * p.D + q.d) * p.N + n] = dA[m][j];
+                if (p.dh0 && q.k == 0) p.dh0[((size_t)q.b * p.D + q.d) * p.N + n] = r[m][j];
+            }
+    }
+    __syncthreads();
+    s_dy[w][lane] = accD;
+    s_dy[4 + w][lane] = accb;
+    __syncthreads();
+    if (w < 2 && q.on) {
+        const float t = (s_dy[w * 4][lane] + s_dy[w * 4 + 1][lane]) + (s_dy[w * 4 + 2][lane] + s_dy[w * 4 + 3][lane]);
+        (w ? p.part_b : p.part_d)[row * p.D + q.d] = t;
+    }
+}
+
+// dB / dC: the parts of a group's channel tiles added in order, written in the activation type at the frame's place
+template <typename TY>
+__global__ __launch_bounds__(256) void sscan_dbc_kernel(const float* __restrict__ part, int T, int B, int N, int NP, int G,
+                                                        int tpg, int reverse, const int* __restrict__ lens, TY* dB, TY* dC) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t per = (size_t)B * T * 2 * NP;
+    if (i >= per) return;
+    const int g = blockIdx.y;
+    const int n = (int)(i % NP), c = (int)(i / NP) & 1;
+    const size_t bs = i / (2 * NP);
+    const int b = (int)(bs / T), s = (int)(bs % T);
+    if (n >= N) return;
+    const int len = row_len(lens, b, T);
+    float v = 0.f;
+    if (s < len)
+        for (int k = 0; k < tpg; ++k) v += part[((size_t)g * tpg + k) * per + i];
+    const long long f = (reverse && s < len) ? len - 1 - s : s;
+    stf((c ? dC : dB) + ((f * B + b) * G + g) * N + n, v);
+}
+
+// ---------------------------------------------------------------- C entry
+struct BwdWs { size_t c_h, c_ds, bc, a, d, b, total; };
+static BwdWs bwd_ws(int T, int B, int D, int N, int G) {
+    const int S = sscan_chunks(T, B, D, N, G, 1), np = sscan_np(N), tpg = (D / G + 63) / 64;
+    BwdWs o{};
+    size_t at = 0;
+    const auto take = [&](size_t floats) { const size_t v = at; at += align256(floats * 4); return v; };
+    o.c_h = take(S > 1 ? (size_t)S * B * np * D : 0);
+    o.c_ds = take(S > 1 ? (size_t)S * B * D : 0);
+    o.bc = take((size_t)G * tpg * B * T * 2 * np);
+    o.a = take((size_t)S * B * D * N);
+    o.d = take((size_t)S * B * D);
+    o.b = take((size_t)S * B * D);
+    o.total = at;
+    return o;
+}
+size_t sscan_bwd_ws(int T, int B, int D, int N, int G) { return bwd_ws(T, B, D, N, G).total; }
+
+template <typename TY, int SPL, int NB>
+static void launch_bwd(const SscanArgs& p, hipStream_t stream) {
+    if (p.S > 1)
+        hipLaunchKernelGGL((sstate_bwd_kernel<TY, SPL, NB, true>), dim3(p.G * p.tpg, p.B, p.S), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((sstate_bwd_kernel<TY, SPL, NB, false>), dim3(p.G * p.tpg, p.B, p.S), dim3(256), 0, stream, p);
+}
+template <typename TY>
+static void launch_bwd_t(const SscanArgs& p, void* dB, void* dC, hipStream_t stream) {
+    if (p.N <= 4) launch_bwd<TY, 1, 1>(p, stream);
+    else if (p.N <= 8) launch_bwd<TY, 2, 1>(p, stream);
+    else if (p.N <= 16) launch_bwd<TY, 4, 1>(p, stream);
+    else if (p.N <= 32) launch_bwd<TY, 4, 2>(p, stream);
+    else launch_bwd<TY, 4, 4>(p, stream);
+    const size_t per = (size_t)p.B * p.T * 2 * p.np;
+    if (per)
+        hipLaunchKernelGGL((sscan_dbc_kernel<TY>), dim3((unsigned)((per + 255) / 256), p.G), dim3(256), 0, stream, p.part_bc,
+                           p.T, p.B, p.N, p.np, p.G, p.tpg, p.reverse, p.lens, (TY*)dB, (TY*)dC);
+}
+
+extern "C" int asr_sscan_bwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes, hipStream_t stream) {
+    SscanArgs p{};
+    if (int e = sscan_fill(d, &p, 1)) return e;
+    if (!d->dA || (d->z && !d->dz && d->T > 0 && d->B > 0)) return ASR_ERR_ARG;
+    if (d->T > 0 && d->B > 0 && (!d->dout || !d->ckpt || !d->dx || !d->ddt || !d->dB || !d->dC)) return ASR_ERR_ARG;
+    if (d->G > 65535) return ASR_ERR_LIMIT;
+    if (d->dh0 && d->dh0 == d->dh_last) return ASR_ERR_ARG;
+    const BwdWs o = bwd_ws(d->T, d->B, d->D, d->N, d->G);
+    if (d->B && (!ws || ws_bytes < o.total)) return ASR_ERR_WS;
+    char* base = (char*)ws;
+    p.c_h = (float*)(base + o.c_h); p.c_ds = (float*)(base + o.c_ds); p.part_bc = (float*)(base + o.bc);
+    p.part_a = (float*)(base + o.a); p.part_d = (float*)(base + o.d); p.part_b = (float*)(base + o.b);
+    int P = 0;
+    if (d->B) {
+        if (d->dtype == ASR_F32) launch_bwd_t<float>(p, d->dB, d->dC, stream);
+        else if (d->dtype == ASR_BF16) launch_bwd_t<bf16_t>(p, d->dB, d->dC, stream);
+        else launch_bwd_t<f16_t>(p, d->dB, d->dC, stream);
+        ASR_CHECK_LAUNCH();
+        P = p.S * p.B;
+    }
+    const size_t n = (size_t)p.D * p.N;
+    sum_partials(p.part_a, n, P, n, d->dA, stream);
+    if (d->dD) sum_partials(p.part_d, p.D, P, p.D, d->dD, stream);
+    if (d->ddt_bias) sum_partials(p.part_b, p.D, P, p.D, d->ddt_bias, stream);
+    ASR_CHECK_LAUNCH();
+    return ASR_OK;
+}

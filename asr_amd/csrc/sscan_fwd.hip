@@ -1,0 +1,300 @@
+#include "sscan.h"
+
+// PRE = false: outputs (and, for training, the state in front of every tile).  PRE = true: only the state a chunk ends in
+// when it starts from zero, and its sum of delta; chunk k of the main pass starts from what these give.
+template <typename TY, int SPL, int NB, bool PRE>
+__global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
+    constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS;
+    __shared__ float2 s_du[TS][64];
+    __shared__ __attribute__((aligned(16))) float s_B[TS][NP];
+    __shared__ __attribute__((aligned(16))) float s_C[PRE ? 1 : TS][NP];
+    __shared__ float s_y[PRE ? 1 : 4][TS][64];
+    const Place q = sscan_place(p);
+    const int tid = threadIdx.x, lane = q.lane, w = q.w;
+    if (PRE && q.t0 >= q.t1) return;
+    const TY* px = (const TY*)p.x + q.b * p.x_sb + q.d;
+    const TY* pdt = (const TY*)p.dt + q.b * p.dt_sb + q.d;
+    const TY* pz = p.z ? (const TY*)p.z + q.b * p.z_sb + q.d : nullptr;
+    const TY* pB = (const TY*)p.Bm + q.b * p.b_sb + q.g * p.b_sg;
+    const TY* pC = (const TY*)p.Cm + q.b * p.c_sb + q.g * p.c_sg;
+    TY* po = (TY*)p.out + q.b * p.o_sb + q.d;
+    const float bias = p.bias ? p.bias[q.d] : 0.f;
+    const float Dk = p.Dk ? p.Dk[q.d] : 0.f;
+    float A2[NB][SPL], h[NB][SPL];
+#pragma unroll
+    for (int m = 0; m < NB; ++m)
+#pragma unroll
+        for (int j = 0; j < SPL; ++j) {
+            const int n = (m * 4 + w) * SPL + j;
+            A2[m][j] = n < p.N ? p.A[(size_t)q.d * p.N + n] * LOG2E : 0.f;
+            h[m][j] = (!PRE && p.h0 && n < p.N) ? p.h0[((size_t)q.b * p.D + q.d) * p.N + n] : 0.f;
+        }
+    if (!PRE) {                       // the state this chunk starts from
+        for (int j = 0; j < q.k && j * p.tpc < q.nt; ++j) {
+            const float ds = p.c_ds[((size_t)j * p.B + q.b) * p.D + q.d];
+#pragma unroll
+            for (int m = 0; m < NB; ++m)
+#pragma unroll
+                for (int i = 0; i < SPL; ++i) {
+                    const int n = (m * 4 + w) * SPL + i;
+                    const float hl = p.c_h[(((size_t)j * p.B + q.b) * NP + n) * p.D + q.d];
+                    h[m][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][i] * ds), h[m][i], hl);
+                }
+        }
+    }
+    float dsum = 0.f;
+    for (int tile = q.t0; tile < q.t1; ++tile) {
+        const int sb = tile * TS;
+        float rx[4], rz[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = sb + w * 4 + i;
+            float de = 0.f;
+            rx[i] = 0.f; rz[i] = 0.f;
+            if (s < q.len) {
+                const long long f = p.reverse ? q.len - 1 - s : s;
+                rx[i] = ldf(px + f * p.x_st);
+                const float v = ldf(pdt + f * p.dt_st) + bias;
+                if (!PRE && pz) rz[i] = ldf(pz + f * p.z_st);
+                de = p.softplus ? softplus_(v) : v;
+            }
+            s_du[w * 4 + i][lane] = float2{de, de * rx[i]};
+        }
+        for (int i = tid; i < TS * NP; i += 256) {
+            const int st = i / NP, n = i % NP, s = sb + st;
+            float vb = 0.f, vc = 0.f;
+            if (s < q.len && n < p.N) {
+                const long long f = p.reverse ? q.len - 1 - s : s;
+                vb = ldf(pB + f * p.b_st + n);
+                if (!PRE) vc = ldf(pC + f * p.c_st + n);
+            }
+            s_B[st][n] = vb;
+            if (!PRE) s_C[st][n] = vc;
+        }
+        __syncthreads();
+        if (!PRE && p.ckpt) {
+            float* ck = p.ckpt + (((size_t)tile * p.B + q.b) * NP) * p.D + q.d;
+            if (q.on)
+#pragma unroll
+                for (int m = 0; m < NB; ++m)
+#pragma unroll
+                    for (int j = 0; j < SPL; ++j) ck[(size_t)((m * 4 + w) * SPL + j) * p.D] = h[m][j];
+        }
+#pragma unroll 4
+        for (int t = 0; t < TS; ++t) {
+            const float2 du = s_du[t][lane];
+            float y = 0.f;
+#pragma unroll
+            for (int m = 0; m < NB; ++m)
+#pragma unroll
+                for (int j = 0; j < SPL; ++j) {
+                    const int n = (m * 4 + w) * SPL + j;
+                    h[m][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][j] * du.x), h[m][j], du.y * s_B[t][n]);
+                    if (!PRE) y = __builtin_fmaf(s_C[t][n], h[m][j], y);
+                }
+            if (!PRE) s_y[w][t][lane] = y;
+            else if (w == 0) dsum += du.x;
+        }
+        __syncthreads();
+        if (!PRE) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = w * 4 + i, s = sb + t;
+                if (s >= p.T || !q.on) continue;
+                float y = ((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i];
+                if (pz) y *= silu_(rz[i]);
+                const bool ok = s < q.len;
+                const long long f = (p.reverse && ok) ? q.len - 1 - s : s;
+                stf(po + f * p.o_st, ok ? y : 0.f);
+            }
+        }
+    }
+    if (PRE) {
+        if (!q.on) return;
+#pragma unroll
+        for (int m = 0; m < NB; ++m)
+#pragma unroll
+            for (int j = 0; j < SPL; ++j)
+                p.c_h[(((size_t)q.k * p.B + q.b) * NP + (m * 4 + w) * SPL + j) * p.D + q.d] = h[m][j];
+        if (w == 0) p.c_ds[((size_t)q.k * p.B + q.b) * p.D + q.d] = dsum;
+        return;
+    }
+    if (!q.on) return;
+    // the last valid tile's chunk (chunk 0 of an empty row) leaves the state
+    const bool last = q.nt == 0 ? q.k == 0 : (q.t0 < q.nt && q.t0 + p.tpc >= q.nt);
+    if (p.h_last && last) {
+#pragma unroll
+        for (int m = 0; m < NB; ++m)
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) {
+                const int n = (m * 4 + w) * SPL + j;
+                if (n < p.N) p.h_last[((size_t)q.b * p.D + q.d) * p.N + n] = h[m][j];
+            }
+    }
+    const int send = min(p.T, (q.t0 + p.tpc) * TS);
+    for (int s = max(q.nt, q.t0) * TS + w; s < send; s += 4) stf(po + (long long)s * p.o_st, 0.f);   // padding
+}
+
+// One frame: thread = 4 states of a channel (one 16-byte access when N is a multiple of 4), LPC lanes per channel join y.
+template <typename TY, int LPC>
+__global__ __launch_bounds__(256) void sscan_step_kernel(SscanArgs p) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t ch = i / LPC;
+    const int l = (int)(i % LPC), n0 = l * 4;
+    if (ch >= (size_t)p.B * p.D) return;             // whole groups of LPC lanes leave together
+    const int b = (int)(ch / p.D), d = (int)(ch % p.D), g = d / p.dpg;
+    float de = ldf((const TY*)p.dt + b * p.dt_sb + d) + (p.bias ? p.bias[d] : 0.f);
+    if (p.softplus) de = softplus_(de);
+    const float x = ldf((const TY*)p.x + b * p.x_sb + d), u = de * x;
+    const TY* pB = (const TY*)p.Bm + b * p.b_sb + g * p.b_sg;
+    const TY* pC = (const TY*)p.Cm + b * p.c_sb + g * p.c_sg;
+    float* h = p.h_last + ch * p.N;
+    const float* A = p.A + (size_t)d * p.N;
+    float y = 0.f;
+    const int m = min(4, p.N - n0);
+    if (p.vec && n0 < p.N) {
+        f32x4 hv = *(f32x4*)(h + n0);
+        const f32x4 av = *(const f32x4*)(A + n0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            hv[e] = __builtin_fmaf(__builtin_amdgcn_exp2f(av[e] * LOG2E * de), hv[e], u * ldf(pB + n0 + e));
+            y = __builtin_fmaf(ldf(pC + n0 + e), hv[e], y);
+        }
+        *(f32x4*)(h + n0) = hv;
+    } else {
+        for (int e = 0; e < m; ++e) {
+            const float v = __builtin_fmaf(__builtin_amdgcn_exp2f(A[n0 + e] * LOG2E * de), h[n0 + e], u * ldf(pB + n0 + e));
+            h[n0 + e] = v;
+            y = __builtin_fmaf(ldf(pC + n0 + e), v, y);
+        }
+    }
+#pragma unroll
+    for (int o = LPC / 2; o > 0; o >>= 1) y += __shfl_xor(y, o);
+    if (l == 0) {
+        if (p.Dk) y += p.Dk[d] * x;
+        if (p.z) y *= silu_(ldf((const TY*)p.z + b * p.z_sb + d));
+        stf((TY*)p.out + b * p.o_sb + d, y);
+    }
+}
+
+// ---------------------------------------------------------------- C entries
+// Chunks of time: one while rows x channel tiles fill the chip, else as many as fill it.
+int sscan_chunks(int T, int B, int D, int N, int G, int backward) {
+    (void)N; (void)backward;
+    const long long wgs = (long long)G * ((D / G + 63) / 64) * B;
+    const int nt = sscan_tiles(T);
+    long long S = wgs ? 512 / wgs : 1;
+    if (S > nt / 4) S = nt / 4;
+    if (S > 64) S = 64;
+    return S < 1 ? 1 : (int)S;
+}
+
+int sscan_fill(const asr_sscan_desc* d, SscanArgs* p, int backward) {
+    if (!d || d->dtype < ASR_F32 || d->dtype > ASR_F16) return ASR_ERR_ARG;
+    if (d->T < 0 || d->B < 0 || d->D <= 0 || d->N <= 0 || d->G <= 0 || d->D % d->G) return ASR_ERR_ARG;
+    if (d->N > 64 || d->B > 65535 || d->D > (1 << 24) || d->T > (1 << 24)) return ASR_ERR_LIMIT;
+    if (!d->A) return ASR_ERR_ARG;
+    const bool any = d->T > 0 && d->B > 0;
+    if (any && (!d->x || !d->dt || !d->Bm || !d->Cm)) return ASR_ERR_ARG;
+    p->T = d->T; p->B = d->B; p->D = d->D; p->N = d->N; p->G = d->G;
+    p->dpg = d->D / d->G; p->tpg = (p->dpg + 63) / 64;
+    p->reverse = d->reverse; p->softplus = d->softplus;
+    p->S = sscan_chunks(d->T, d->B, d->D, d->N, d->G, backward);
+    p->tpc = (sscan_tiles(d->T) + p->S - 1) / p->S;
+    if (p->tpc < 1) p->tpc = 1;
+    p->np = sscan_np(d->N);
+    p->lens = d->lens;
+    p->x = d->x; p->x_st = d->x_st; p->x_sb = d->x_sb;
+    p->dt = d->dt; p->dt_st = d->dt_st; p->dt_sb = d->dt_sb;
+    p->z = d->z; p->z_st = d->z_st; p->z_sb = d->z_sb;
+    p->Bm = d->Bm; p->b_st = d->b_st; p->b_sb = d->b_sb; p->b_sg = d->b_sg;
+    p->Cm = d->Cm; p->c_st = d->c_st; p->c_sb = d->c_sb; p->c_sg = d->c_sg;
+    p->A = d->A; p->Dk = d->Dk; p->bias = d->dt_bias; p->h0 = d->h0;
+    p->out = d->out; p->o_st = d->o_st; p->o_sb = d->o_sb;
+    p->h_last = d->h_last; p->ckpt = d->ckpt;
+    p->dout = d->dout; p->do_st = d->do_st; p->do_sb = d->do_sb; p->dh_last = d->dh_last;
+    p->dx = d->dx; p->ddt = d->ddt; p->dz = d->dz; p->dh0 = d->dh0;
+    return ASR_OK;
+}
+
+extern "C" size_t asr_sscan_ckpt_floats(int T, int B, int D, int N) {
+    if (T <= 0 || B <= 0 || D <= 0 || N <= 0 || N > 64) return 0;
+    return (size_t)sscan_tiles(T) * B * sscan_np(N) * D;
+}
+
+static size_t fwd_ws(int T, int B, int D, int N, int G) {
+    const int S = sscan_chunks(T, B, D, N, G, 0);
+    return S > 1 ? align256((size_t)S * B * sscan_np(N) * D * 4) + (size_t)S * B * D * 4 : 0;
+}
+
+size_t sscan_bwd_ws(int T, int B, int D, int N, int G);
+extern "C" size_t asr_sscan_ws_bytes(int T, int B, int D, int N, int G, int backward) {
+    if (T <= 0 || B <= 0 || D <= 0 || N <= 0 || N > 64 || G <= 0 || D % G) return 0;
+    return backward ? sscan_bwd_ws(T, B, D, N, G) : fwd_ws(T, B, D, N, G);
+}
+
+template <typename TY, int SPL, int NB>
+static void launch_fwd(const SscanArgs& p, hipStream_t stream) {
+    if (p.S > 1)
+        hipLaunchKernelGGL((sstate_fwd_kernel<TY, SPL, NB, true>), dim3(p.G * p.tpg, p.B, p.S - 1), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((sstate_fwd_kernel<TY, SPL, NB, false>), dim3(p.G * p.tpg, p.B, p.S), dim3(256), 0, stream, p);
+}
+template <typename TY>
+static void launch_fwd_t(const SscanArgs& p, hipStream_t stream) {
+    if (p.N <= 4) launch_fwd<TY, 1, 1>(p, stream);
+    else if (p.N <= 8) launch_fwd<TY, 2, 1>(p, stream);
+    else if (p.N <= 16) launch_fwd<TY, 4, 1>(p, stream);
+    else if (p.N <= 32) launch_fwd<TY, 4, 2>(p, stream);
+    else launch_fwd<TY, 4, 4>(p, stream);
+}
+
+extern "C" int asr_sscan_fwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes, hipStream_t stream) {
+    SscanArgs p{};
+    if (int e = sscan_fill(d, &p, 0)) return e;
+    if (d->h_last && d->h_last == d->h0) return ASR_ERR_ARG;
+    if (d->T > 0 && d->B > 0 && !d->out) return ASR_ERR_ARG;
+    if (d->B == 0 || (d->T == 0 && !d->h_last)) return ASR_OK;
+    if (p.S > 1) {
+        if (!ws || ws_bytes < fwd_ws(d->T, d->B, d->D, d->N, d->G)) return ASR_ERR_WS;
+        p.c_h = (float*)ws;
+        p.c_ds = (float*)((char*)ws + align256((size_t)p.S * p.B * p.np * p.D * 4));
+    }
+    if (d->dtype == ASR_F32) launch_fwd_t<float>(p, stream);
+    else if (d->dtype == ASR_BF16) launch_fwd_t<bf16_t>(p, stream);
+    else launch_fwd_t<f16_t>(p, stream);
+    ASR_CHECK_LAUNCH();
+    return ASR_OK;
+}
+
+template <typename TY>
+static void launch_step(const SscanArgs& p, hipStream_t stream) {
+    const int need = (p.N + 3) / 4;
+    const int lpc = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need <= 8 ? 8 : 16;
+    const dim3 grid((unsigned)(((size_t)p.B * p.D * lpc + 255) / 256));
+#define STEP_(L) hipLaunchKernelGGL((sscan_step_kernel<TY, L>), grid, dim3(256), 0, stream, p)
+    switch (lpc) { case 1: STEP_(1); break; case 2: STEP_(2); break; case 4: STEP_(4); break; case 8: STEP_(8); break;
+                   default: STEP_(16); }
+#undef STEP_
+}
+
+extern "C" int asr_sscan_step(int dtype, int B, int D, int N, int G, float* h, const void* x, long long x_sb, const void* dt,
+                              long long dt_sb, const float* A, const void* Bm, long long b_sb, long long b_sg,
+                              const void* Cm, long long c_sb, long long c_sg, const float* Dk, const void* z,
+                              long long z_sb, const float* dt_bias, int softplus, void* out, long long o_sb,
+                              hipStream_t stream) {
+    if (dtype < ASR_F32 || dtype > ASR_F16 || B < 0 || D <= 0 || N <= 0 || G <= 0 || D % G || !A) return ASR_ERR_ARG;
+    if (N > 64 || B > 65535 || D > (1 << 24)) return ASR_ERR_LIMIT;
+    if (!B) return ASR_OK;
+    if (!h || !x || !dt || !Bm || !Cm || !out) return ASR_ERR_ARG;
+    SscanArgs p{};
+    p.vec = (N & 3) == 0 && !(((uintptr_t)h | (uintptr_t)A) & 15);
+    p.B = B; p.D = D; p.N = N; p.G = G; p.dpg = D / G; p.softplus = softplus;
+    p.x = x; p.x_sb = x_sb; p.dt = dt; p.dt_sb = dt_sb; p.A = A; p.Bm = Bm; p.b_sb = b_sb; p.b_sg = b_sg;
+    p.Cm = Cm; p.c_sb = c_sb; p.c_sg = c_sg; p.Dk = Dk; p.z = z; p.z_sb = z_sb; p.bias = dt_bias; p.h_last = h;
+    p.out = out; p.o_sb = o_sb;
+    if (dtype == ASR_F32) launch_step<float>(p, stream);
+    else if (dtype == ASR_BF16) launch_step<bf16_t>(p, stream);
+    else launch_step<f16_t>(p, stream);
+    ASR_CHECK_LAUNCH();
+    return ASR_OK;
+}

@@ -254,3 +254,8 @@ def lstm_pack(W, N, mode, out):
     assert W.is_contiguous() and out.numel() >= _lib.lib().asr_lstm_pack_floats(N, mode)
     check(_lib.lib().asr_lstm_pack_w(_p(W), N, mode, _p(out), _s()), 'asr_lstm_pack_w')
     return out
+
+
+# the state-space layer's operators
+from .ops_ssm import (causal_conv_fwd, causal_conv_bwd, causal_conv_step, selective_scan_fwd, selective_scan_bwd,  # noqa: E402,F401
+                      selective_scan_step, add_rms_norm_fwd, add_rms_norm_bwd, clip_list)

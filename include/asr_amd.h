@@ -410,6 +410,81 @@ int asr_scaling_bwd(const asr_scaling_desc* d, void* ws, size_t ws_bytes, asr_st
  * that gave up is reported by asr_scan_status(ws, 1).  No counterpart in the reference. */
 int asr_scaling_set_mode(int mode);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * The operators of a selective state-space layer and of its training.  No counterpart in the reference (its recurrences
+ * are LSTMs).  Differences from the conventions above: activations are f32, bf16 or f16 (dtype 0, 1, 2; one type per
+ * call), computed in f32 and rounded once when stored; activation pointers come with strides in elements (_st per frame,
+ * _sb per batch row, _sg per group), channels contiguous; parameters, scan states and parameter gradients are f32 and
+ * contiguous.  lens (B, or NULL = T everywhere): frames at and behind lens[b] are padding, their values are not used,
+ * outputs and gradients there are zero; lens are clamped to [0, T] on the device.  reverse != 0 walks a row's valid frames from the last to the
+ * first.  Buffers written must not overlap any other buffer of the call.  All sums run in a fixed order.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* Short causal depthwise convolution over time, 2 <= K <= 8 taps (ASR_ERR_LIMIT above):
+ *   out[s,b,d] = act(bias[d] + sum_k w[d,k] x[s-(K-1)+k,b,d]),  act != 0: silu.
+ * s counts valid frames in walking order; state (K-1,B,D), in the activations' type, holds the frames s = -(K-1)..-1 (NULL:
+ * zeros), state_out receives the last K-1 frames (may be NULL, must not be state).  The step entry takes one frame and
+ * moves state on in place.  dwb = D*K values of dw, then D of dbias. */
+int asr_conv_fwd(int dtype, int T, int B, int D, int K, const void* x, long long x_st, long long x_sb, const float* w,
+                 const float* bias, const void* state, const int* lens, int act, int reverse, void* out, long long o_st,
+                 long long o_sb, void* state_out, asr_stream_t stream);
+size_t asr_conv_bwd_ws_bytes(int T, int B, int D, int K);
+int asr_conv_bwd(int dtype, int T, int B, int D, int K, const void* dout, long long do_st, long long do_sb, const void* x,
+                 long long x_st, long long x_sb, const float* w, const float* bias, const void* state, const int* lens,
+                 int act, int reverse, const void* dstate_out, void* dx, float* dwb, void* dstate, void* ws,
+                 size_t ws_bytes, asr_stream_t stream);
+int asr_conv_step(int dtype, int B, int D, int K, const void* x, long long x_sb, void* state, const float* w,
+                  const float* bias, int act, void* out, long long o_sb, asr_stream_t stream);
+
+/* Selective scan: delta = softplus(dt + dt_bias) (softplus = 0: dt + dt_bias),
+ *   h[s] = exp(delta A) h[s-1] + delta x B[s],   y = sum_n C[s] h[s] + Dk x,   out = y silu(z)  (z NULL: y)
+ * x, dt, z, out (T,B,D); A (D,N), N <= 64 (ASR_ERR_LIMIT above); Bm, Cm (T,B,G,N), a group's D/G channels share them; Dk,
+ * dt_bias (D) or NULL; h0, h_last (B,D,N) or NULL.  For training the forward call is given ckpt (asr_sscan_ckpt_floats) and
+ * the backward call the same descriptor with ckpt as the forward call left it.  Backward outputs: dx, ddt, dz (T,B,D) and
+ * dB, dC (T,B,G,N) contiguous in the activations' type; dA (D,N), dD (D), ddt_bias (D), dh0 (B,D,N) f32; dz, dD, ddt_bias, dh0
+ * may be NULL where there is nothing to differentiate.  ws: asr_sscan_ws_bytes (0 bytes: NULL will do).  The step entry takes one frame, h (B,D,N) moves on in place. */
+typedef struct asr_sscan_desc {
+    int T, B, D, N, G, dtype, reverse, softplus;
+    const int* lens;
+    const void* x; long long x_st, x_sb;
+    const void* dt; long long dt_st, dt_sb;
+    const void* z; long long z_st, z_sb;
+    const void* Bm; long long b_st, b_sb, b_sg;
+    const void* Cm; long long c_st, c_sb, c_sg;
+    const float *A, *Dk, *dt_bias, *h0;
+    void* out; long long o_st, o_sb;
+    float *h_last, *ckpt;
+    const void* dout; long long do_st, do_sb;   /* backward in */
+    const float* dh_last;                       /* backward in: gradient of h_last, or NULL */
+    void *dx, *ddt, *dz, *dB, *dC;              /* backward out */
+    float *dA, *dD, *ddt_bias, *dh0;
+} asr_sscan_desc;
+size_t asr_sscan_ckpt_floats(int T, int B, int D, int N);
+size_t asr_sscan_ws_bytes(int T, int B, int D, int N, int G, int backward);
+int asr_sscan_fwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes, asr_stream_t stream);
+int asr_sscan_bwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes, asr_stream_t stream);
+int asr_sscan_step(int dtype, int B, int D, int N, int G, float* h, const void* x, long long x_sb, const void* dt,
+                   long long dt_sb, const float* A, const void* Bm, long long b_sb, long long b_sg, const void* Cm,
+                   long long c_sb, long long c_sg, const float* Dk, const void* z, long long z_sb, const float* dt_bias,
+                   int softplus, void* out, long long o_sb, asr_stream_t stream);
+
+/* r = x (+ res), y = r rstd w, rstd = 1 / sqrt(mean(r^2) + eps) over rows of n columns (leading dimensions ldx, ldr, in
+ * elements).  sum (rows,n) receives r, rstd (rows) the factors; both may be NULL.  Backward: x and res as the forward
+ * call had them, dres (or NULL) the gradient that reaches r directly; dx = d r, the gradient of x and of res. */
+int asr_rms_norm_fwd(int dtype, const void* x, long long ldx, const void* res, long long ldr, const float* w, int rows,
+                     int n, float eps, void* y, void* sum, float* rstd, asr_stream_t stream);
+size_t asr_rms_norm_bwd_ws_bytes(int rows, int n);
+int asr_rms_norm_bwd(int dtype, const void* dy, long long lddy, const void* x, long long ldx, const void* res,
+                     long long ldr, const float* w, const float* rstd, const void* dres, long long ldd, int rows, int n, void* dx, float* dw, void* ws,
+                     size_t ws_bytes, asr_stream_t stream);
+
+/* total_norm_constraint (libs/lasagne_libs/updates.py:781-855) for gradients in `count` separate contiguous buffers of
+ * dtypes[i] and sizes[i] elements (0 allowed): norm_out[0] = sqrt(sum of all squares, in double), dst[i] = src[i] *
+ * clip(norm, 0, max_norm) / (eps + norm).  dst[i] may be src[i].  The four arrays are host memory and are read before the call returns. */
+size_t asr_clip_list_ws_bytes(int count, const long long* sizes);
+int asr_clip_list(int count, const int* dtypes, const void* const* src, void* const* dst, const long long* sizes,
+                  float max_norm, float eps, float* norm_out, void* ws, size_t ws_bytes, asr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
