@@ -333,7 +333,7 @@ def _own_norm(s):
     y, r, rstd = ops.add_rms_norm_fwd(s['x'], s['w'], residual=s['res'], eps=EPS)
     if s['mode'] != 'train':
         return [y, r]
-    dx, dw = ops.add_rms_norm_bwd(s['dy'], r, s['w'], rstd, dres=s['dres'])
+    dx, dw = ops.add_rms_norm_bwd(s['dy'], s['x'], s['w'], rstd, residual=s['res'], dres=s['dres'])
     return [y, r, dx, dw]
 
 
