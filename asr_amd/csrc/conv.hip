@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p, int run) {
                     float a = bias[e];
 #pragma unroll
                     for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][e], win[k][e], a);
-                    if (p.act) g[e] *= dsilu_(a, sigmoidf_(a));
+                    if (p.act) g[e] *= dsilu_(a, sigm_(a));
                     dp[K - 1][e] = g[e];
                     if (q < own) {
 #pragma unroll

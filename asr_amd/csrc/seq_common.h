@@ -34,11 +34,33 @@ template <typename T, int V> __device__ __forceinline__ void stv(T* p, const flo
     }
 }
 
-__device__ __forceinline__ float silu_(float z) { return z * sigmoidf_(z); }
+// e^-|v| in (0, 1]: the argument's product with log2 e in two floats, the rest as a first-order correction; a NaN stays one.
+__device__ __forceinline__ float exp_neg_abs_(float v) {
+    const float L2E_HI = 0x1.715476p+0f, L2E_LO = 0x1.4ae0c0p-26f, LN2_ = 0x1.62e430p-1f;
+    float x = -fabsf(v);
+    x = x < -110.0f ? -110.0f : x;
+    const float hi = x * L2E_HI, lo = __builtin_fmaf(x, L2E_HI, -hi) + x * L2E_LO;
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return __builtin_fmaf(e, lo * LN2_, e);
+}
+// 1 / (1 + e^-v) from u = e^-|v|: the divisor lies in [1, 2], so a reciprocal and one Newton step serve
+__device__ __forceinline__ float sigmoid_from_(float v, float u) {
+    const float d = 1.0f + u, r = __builtin_amdgcn_rcpf(d);
+    const float rr = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+    return v < 0.0f ? u * rr : rr;
+}
+__device__ __forceinline__ float sigm_(float v) { return sigmoid_from_(v, exp_neg_abs_(v)); }
+__device__ __forceinline__ float silu_(float z) { return z * sigm_(z); }
 // d silu / dz, from z and its sigmoid
 __device__ __forceinline__ float dsilu_(float z, float sg) { return sg * (1.0f + z * (1.0f - sg)); }
-// log(1 + e^v) without overflow and with relative accuracy for very negative v
-__device__ __forceinline__ float softplus_(float v) { return fmaxf(v, 0.0f) + log1pf(expf_(-fabsf(v))); }
+// log(1 + e^v) = max(v, 0) + log1p(u), u = e^-|v|: no overflow, relative accuracy for very negative v.  log1p(u) = log(w) u / (w - 1)
+// with w = 1 + u rounded (Kahan's form: the rounding of w is in both factors), u itself where w = 1.
+__device__ __forceinline__ float softplus_from_(float v, float u) {
+    const float w = 1.0f + u, d = w - 1.0f;
+    const float l = __builtin_amdgcn_logf(w) * 0x1.62e430p-1f;
+    return (v < 0.0f ? 0.0f : v) + (d == 0.0f ? u : l * (u * __builtin_amdgcn_rcpf(d)));
+}
+__device__ __forceinline__ float softplus_(float v) { return softplus_from_(v, exp_neg_abs_(v)); }
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

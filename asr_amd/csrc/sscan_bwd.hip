@@ -198,12 +198,12 @@ __global__ __launch_bounds__(256) void sstate_bwd_kernel(SscanArgs p) {
             const long long f = (p.reverse && ok) ? q.len - 1 - s : s;
             const size_t o = f * ostep + obase;
             float ddt = __builtin_fmaf(rx[i], s1, s2 * LN2);
-            if (p.softplus) ddt *= sigmoidf_(rr[i]);
+            if (p.softplus) ddt *= sigm_(rr[i]);
             stf((TY*)p.dx + o, ok ? __builtin_fmaf(rd[i], s1, Dk * ry[i]) : 0.f);
             stf((TY*)p.ddt + o, ok ? ddt : 0.f);
             if (pz) {
                 const float y = ((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i];
-                stf((TY*)p.dz + o, ok ? rg[i] * y * dsilu_(rz[i], sigmoidf_(rz[i])) : 0.f);
+                stf((TY*)p.dz + o, ok ? rg[i] * y * dsilu_(rz[i], sigm_(rz[i])) : 0.f);
             }
             if (ok) { accD = __builtin_fmaf(ry[i], rx[i], accD); accb += ddt; }
         }

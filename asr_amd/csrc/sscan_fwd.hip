@@ -2,124 +2,157 @@
 
 // PRE = false: outputs (and, for training, the state in front of every tile).  PRE = true: only the state a chunk ends in
 // when it starts from zero, and its sum of delta; chunk k of the main pass starts from what these give.
+//
+// One barrier a tile: while a tile's states are walked, the next tile's delta, delta x, B and C go into the other half of the
+// LDS buffers and the tile after that is on its way from memory into registers.
 template <typename TY, int SPL, int NB, bool PRE>
 __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
-    constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS;
-    __shared__ float2 s_du[TS][64];
-    __shared__ __attribute__((aligned(16))) float s_B[TS][NP];
-    __shared__ __attribute__((aligned(16))) float s_C[PRE ? 1 : TS][NP];
-    __shared__ float s_y[PRE ? 1 : 4][TS][64];
+    constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RB = (TS * NP + 255) / 256;
+    __shared__ float2 s_du[2][TS][64];
+    __shared__ __attribute__((aligned(16))) float s_B[2][TS * NP];
+    __shared__ __attribute__((aligned(16))) float s_C[2][PRE ? 1 : TS * NP];
+    __shared__ float s_y[2][PRE ? 1 : 4][PRE ? 1 : TS][64];
     const Place q = sscan_place(p);
     const int tid = threadIdx.x, lane = q.lane, w = q.w;
     if (PRE && q.t0 >= q.t1) return;
-    const TY* px = (const TY*)p.x + q.b * p.x_sb + q.d;
-    const TY* pdt = (const TY*)p.dt + q.b * p.dt_sb + q.d;
-    const TY* pz = p.z ? (const TY*)p.z + q.b * p.z_sb + q.d : nullptr;
+    const TY* px = (const TY*)p.x + q.b * p.x_sb;
+    const TY* pdt = (const TY*)p.dt + q.b * p.dt_sb;
+    const TY* pz = p.z ? (const TY*)p.z + q.b * p.z_sb : nullptr;
     const TY* pB = (const TY*)p.Bm + q.b * p.b_sb + q.g * p.b_sg;
     const TY* pC = (const TY*)p.Cm + q.b * p.c_sb + q.g * p.c_sg;
-    TY* po = (TY*)p.out + q.b * p.o_sb + q.d;
-    const float bias = p.bias ? p.bias[q.d] : 0.f;
-    const float Dk = p.Dk ? p.Dk[q.d] : 0.f;
+    TY* po = (TY*)p.out + q.b * p.o_sb;
+    const unsigned d = q.d;
+    const float bias = p.bias ? p.bias[d] : 0.f;
+    const float Dk = p.Dk ? p.Dk[d] : 0.f;
     float A2[NB][SPL], h[NB][SPL];
 #pragma unroll
     for (int m = 0; m < NB; ++m)
 #pragma unroll
         for (int j = 0; j < SPL; ++j) {
             const int n = (m * 4 + w) * SPL + j;
-            A2[m][j] = n < p.N ? p.A[(size_t)q.d * p.N + n] * LOG2E : 0.f;
-            h[m][j] = (!PRE && p.h0 && n < p.N) ? p.h0[((size_t)q.b * p.D + q.d) * p.N + n] : 0.f;
+            A2[m][j] = n < p.N ? p.A[(size_t)d * p.N + n] * LOG2E : 0.f;
+            h[m][j] = (!PRE && p.h0 && n < p.N) ? p.h0[((size_t)q.b * p.D + d) * p.N + n] : 0.f;
         }
     if (!PRE) {                       // the state this chunk starts from
         for (int j = 0; j < q.k && j * p.tpc < q.nt; ++j) {
-            const float ds = p.c_ds[((size_t)j * p.B + q.b) * p.D + q.d];
+            const float ds = p.c_ds[((size_t)j * p.B + q.b) * p.D + d];
 #pragma unroll
             for (int m = 0; m < NB; ++m)
 #pragma unroll
                 for (int i = 0; i < SPL; ++i) {
                     const int n = (m * 4 + w) * SPL + i;
-                    const float hl = p.c_h[(((size_t)j * p.B + q.b) * NP + n) * p.D + q.d];
+                    const float hl = p.c_h[(((size_t)j * p.B + q.b) * NP + n) * p.D + d];
                     h[m][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][i] * ds), h[m][i], hl);
                 }
         }
     }
     float dsum = 0.f;
-    for (int tile = q.t0; tile < q.t1; ++tile) {
-        const int sb = tile * TS;
-        float rx[4], rz[4];
+    TY lx[4], ldt[4], lz[4], lB[RB], lC[RB];        // on their way: own frames w*4 .. w*4+3 of a tile, own part of B and C
+    float rx[4], rz[4], nx[4], nz[4];               // x, z of the tile being walked and of the next
+    const auto frame = [&](int s) -> long long {    // clamped: what is read behind the row is thrown away below
+        s = min(s, q.len - 1);
+        return p.reverse ? q.len - 1 - s : s;
+    };
+    const auto fetch = [&](int tile) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = sb + w * 4 + i;
-            float de = 0.f;
-            rx[i] = 0.f; rz[i] = 0.f;
-            if (s < q.len) {
-                const long long f = p.reverse ? q.len - 1 - s : s;
-                rx[i] = ldf(px + f * p.x_st);
-                const float v = ldf(pdt + f * p.dt_st) + bias;
-                if (!PRE && pz) rz[i] = ldf(pz + f * p.z_st);
-                de = p.softplus ? softplus_(v) : v;
-            }
-            s_du[w * 4 + i][lane] = float2{de, de * rx[i]};
+            const long long f = frame(tile * TS + w * 4 + i);
+            lx[i] = (px + f * p.x_st)[d];
+            ldt[i] = (pdt + f * p.dt_st)[d];
+            if (!PRE && pz) lz[i] = (pz + f * p.z_st)[d];
         }
-        for (int i = tid; i < TS * NP; i += 256) {
-            const int st = i / NP, n = i % NP, s = sb + st;
-            float vb = 0.f, vc = 0.f;
-            if (s < q.len && n < p.N) {
-                const long long f = p.reverse ? q.len - 1 - s : s;
-                vb = ldf(pB + f * p.b_st + n);
-                if (!PRE) vc = ldf(pC + f * p.c_st + n);
+#pragma unroll
+        for (int k = 0; k < RB; ++k) {
+            const int e = tid + k * 256;
+            const long long f = frame(tile * TS + e / NP);
+            const int n = min(e % NP, p.N - 1);
+            if (RB * 256 == TS * NP || e < TS * NP) {
+                lB[k] = (pB + f * p.b_st)[n];
+                if (!PRE) lC[k] = (pC + f * p.c_st)[n];
             }
-            s_B[st][n] = vb;
-            if (!PRE) s_C[st][n] = vc;
         }
+    };
+    const auto place = [&](int tile, int half) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool ok = tile * TS + w * 4 + i < q.len;
+            const float v = (float)ldt[i] + bias;
+            const float de = ok ? (p.softplus ? softplus_(v) : v) : 0.f;
+            nx[i] = ok ? (float)lx[i] : 0.f;
+            nz[i] = (!PRE && pz && ok) ? (float)lz[i] : 0.f;
+            s_du[half][w * 4 + i][lane] = float2{de, de * nx[i]};
+        }
+#pragma unroll
+        for (int k = 0; k < RB; ++k) {
+            const int e = tid + k * 256;
+            if (RB * 256 == TS * NP || e < TS * NP) {
+                const bool ok = tile * TS + e / NP < q.len && e % NP < p.N;
+                s_B[half][e] = ok ? (float)lB[k] : 0.f;
+                if (!PRE) s_C[half][e] = ok ? (float)lC[k] : 0.f;
+            }
+        }
+    };
+    if (q.t0 < q.t1) {
+        fetch(q.t0);
+        place(q.t0, 0);
+        fetch(min(q.t0 + 1, q.t1 - 1));
         __syncthreads();
-        if (!PRE && p.ckpt) {
-            float* ck = p.ckpt + (((size_t)tile * p.B + q.b) * NP) * p.D + q.d;
-            if (q.on)
+    }
+    for (int tile = q.t0; tile < q.t1; ++tile) {
+        const int half = (tile - q.t0) & 1, sb = tile * TS;
 #pragma unroll
-                for (int m = 0; m < NB; ++m)
+        for (int i = 0; i < 4; ++i) { rx[i] = nx[i]; rz[i] = nz[i]; }
+        if (!PRE && p.ckpt && q.on) {
+            float* ck = p.ckpt + (((size_t)tile * p.B + q.b) * NP + w * SPL) * p.D;
 #pragma unroll
-                    for (int j = 0; j < SPL; ++j) ck[(size_t)((m * 4 + w) * SPL + j) * p.D] = h[m][j];
+            for (int m = 0; m < NB; ++m)
+#pragma unroll
+                for (int j = 0; j < SPL; ++j) (ck + (size_t)(m * 4 * SPL + j) * p.D)[d] = h[m][j];
         }
-#pragma unroll 4
+#pragma unroll
         for (int t = 0; t < TS; ++t) {
-            const float2 du = s_du[t][lane];
+            const float2 du = s_du[half][t][lane];
             float y = 0.f;
 #pragma unroll
             for (int m = 0; m < NB; ++m)
 #pragma unroll
                 for (int j = 0; j < SPL; ++j) {
-                    const int n = (m * 4 + w) * SPL + j;
-                    h[m][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][j] * du.x), h[m][j], du.y * s_B[t][n]);
-                    if (!PRE) y = __builtin_fmaf(s_C[t][n], h[m][j], y);
+                    const int e = t * NP + (m * 4 + w) * SPL + j;
+                    h[m][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][j] * du.x), h[m][j], du.y * s_B[half][e]);
+                    if (!PRE) y = __builtin_fmaf(s_C[half][e], h[m][j], y);
                 }
-            if (!PRE) s_y[w][t][lane] = y;
+            if (!PRE) s_y[half][w][t][lane] = y;
             else if (w == 0) dsum += du.x;
         }
+        if (tile + 1 < q.t1) {
+            place(tile + 1, half ^ 1);
+            fetch(min(tile + 2, q.t1 - 1));
+        }
         __syncthreads();
-        if (!PRE) {
+        if (!PRE && q.on) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = w * 4 + i, s = sb + t;
-                if (s >= p.T || !q.on) continue;
-                float y = ((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i];
+                if (s >= p.T) continue;
+                float y = ((s_y[half][0][t][lane] + s_y[half][1][t][lane]) +
+                           (s_y[half][2][t][lane] + s_y[half][3][t][lane])) + Dk * rx[i];
                 if (pz) y *= silu_(rz[i]);
                 const bool ok = s < q.len;
                 const long long f = (p.reverse && ok) ? q.len - 1 - s : s;
-                stf(po + f * p.o_st, ok ? y : 0.f);
+                (po + f * p.o_st)[d] = (TY)(ok ? y : 0.f);
             }
         }
     }
+    if (!q.on) return;
     if (PRE) {
-        if (!q.on) return;
 #pragma unroll
         for (int m = 0; m < NB; ++m)
 #pragma unroll
             for (int j = 0; j < SPL; ++j)
-                p.c_h[(((size_t)q.k * p.B + q.b) * NP + (m * 4 + w) * SPL + j) * p.D + q.d] = h[m][j];
-        if (w == 0) p.c_ds[((size_t)q.k * p.B + q.b) * p.D + q.d] = dsum;
+                p.c_h[(((size_t)q.k * p.B + q.b) * NP + (m * 4 + w) * SPL + j) * p.D + d] = h[m][j];
+        if (w == 0) p.c_ds[((size_t)q.k * p.B + q.b) * p.D + d] = dsum;
         return;
     }
-    if (!q.on) return;
     // the last valid tile's chunk (chunk 0 of an empty row) leaves the state
     const bool last = q.nt == 0 ? q.k == 0 : (q.t0 < q.nt && q.t0 + p.tpc >= q.nt);
     if (p.h_last && last) {
@@ -128,11 +161,11 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
 #pragma unroll
             for (int j = 0; j < SPL; ++j) {
                 const int n = (m * 4 + w) * SPL + j;
-                if (n < p.N) p.h_last[((size_t)q.b * p.D + q.d) * p.N + n] = h[m][j];
+                if (n < p.N) p.h_last[((size_t)q.b * p.D + d) * p.N + n] = h[m][j];
             }
     }
     const int send = min(p.T, (q.t0 + p.tpc) * TS);
-    for (int s = max(q.nt, q.t0) * TS + w; s < send; s += 4) stf(po + (long long)s * p.o_st, 0.f);   // padding
+    for (int s = max(q.nt, q.t0) * TS + w; s < send; s += 4) (po + (long long)s * p.o_st)[d] = (TY)0.f;   // padding
 }
 
 // One frame: thread = 4 states of a channel (one 16-byte access when N is a multiple of 4), LPC lanes per channel join y.
