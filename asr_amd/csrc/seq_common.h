@@ -34,11 +34,11 @@ template <typename T, int V> __device__ __forceinline__ void stv(T* p, const flo
     }
 }
 
-// e^-|v| in (0, 1]: the argument's product with log2 e in two floats, the rest as a first-order correction; a NaN stays one.
+// e^-|v| in (0, 1]: the argument's product with log2 e in two floats, the rest as a first-order correction.  Finite for
+// every v (a NaN becomes e^-110): the functions below carry v itself on, and with it infinities and NaN.
 __device__ __forceinline__ float exp_neg_abs_(float v) {
     const float L2E_HI = 0x1.715476p+0f, L2E_LO = 0x1.4ae0c0p-26f, LN2_ = 0x1.62e430p-1f;
-    float x = -fabsf(v);
-    x = x < -110.0f ? -110.0f : x;
+    const float x = fmaxf(-fabsf(v), -110.0f);
     const float hi = x * L2E_HI, lo = __builtin_fmaf(x, L2E_HI, -hi) + x * L2E_LO;
     const float e = __builtin_amdgcn_exp2f(hi);
     return __builtin_fmaf(e, lo * LN2_, e);

@@ -67,3 +67,64 @@ __device__ __forceinline__ Place sscan_place(const SscanArgs& p) {
     q.t1 = min(q.t0 + p.tpc, q.nt);                     // this chunk's tiles; none if t1 <= t0
     return q;
 }
+
+// A thread's share of a tile's rows: frames w*4 .. w*4+3 of its channel.  `base` is the row's own address (uniform), `off` the
+// channel's byte offset, so an access is a scalar address plus a 32-bit lane offset.  FULL: all frames are valid.  Otherwise
+// frames behind the row read its last one, and what they give is thrown away by the caller.
+template <bool FULL, typename TY>
+__device__ __forceinline__ void fetch_rows(TY (&o)[4], const TY* base, long long st, int s0, int len, int reverse, unsigned off) {
+    const char* b = (const char*)base;
+    const long long sb = st * (long long)sizeof(TY);
+    if (FULL) {
+        const char* r = b + (long long)(reverse ? len - 1 - s0 : s0) * sb;
+        const long long step = reverse ? -sb : sb;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { o[i] = *(const TY*)(r + off); r += step; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = min(s0 + i, len - 1);
+            o[i] = *(const TY*)(b + (long long)(reverse ? len - 1 - s : s) * sb + off);
+        }
+    }
+}
+// The same frames of an output: padding rows in front of p.T get zeros.
+template <bool FULL, typename TY>
+__device__ __forceinline__ void store_rows(TY* base, long long st, int s0, int len, int T, int reverse, unsigned off,
+                                           const float (&v)[4]) {
+    char* b = (char*)base;
+    const long long sb = st * (long long)sizeof(TY);
+    if (FULL) {
+        char* r = b + (long long)(reverse ? len - 1 - s0 : s0) * sb;
+        const long long step = reverse ? -sb : sb;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { *(TY*)(r + off) = (TY)v[i]; r += step; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i;
+            const bool ok = s < len;
+            if (s < T) *(TY*)(b + (long long)((reverse && ok) ? len - 1 - s : s) * sb + off) = (TY)(ok ? v[i] : 0.f);
+        }
+    }
+}
+// Its share of B and C: TS frames x NP states, one value every 256 of them.
+template <typename TY, int NP, int RB>
+__device__ __forceinline__ void fetch_states(TY (&o)[RB], const TY* base, long long st, int tile, int len, int reverse, int N) {
+#pragma unroll
+    for (int k = 0; k < RB; ++k) {
+        const int e = threadIdx.x + k * 256;
+        const int s = min(tile * SSCAN_TS + min(e / NP, SSCAN_TS - 1), len - 1);
+        o[k] = base[(reverse ? len - 1 - s : s) * st + min(e % NP, N - 1)];
+    }
+}
+template <typename TY, int NP, int RB>
+__device__ __forceinline__ void place_states(float* dst, const TY (&o)[RB], int tile, int len, int N) {
+#pragma unroll
+    for (int k = 0; k < RB; ++k) {
+        const int e = threadIdx.x + k * 256;
+        if (RB * 256 == SSCAN_TS * NP || e < SSCAN_TS * NP)
+            dst[e] = (tile * SSCAN_TS + e / NP < len && e % NP < N) ? (float)o[k] : 0.f;
+    }
+}
+template <bool V> struct Flag { static constexpr bool value = V; };

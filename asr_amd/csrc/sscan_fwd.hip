@@ -47,67 +47,50 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
         }
     }
     float dsum = 0.f;
-    TY lx[4], ldt[4], lz[4], lB[RB], lC[RB];        // on their way: own frames w*4 .. w*4+3 of a tile, own part of B and C
+    // on their way from memory: own frames w*4 .. w*4+3 of a tile, own part of B and C
+    TY lx[4], ldt[4], lz[4], lB[RB], lC[RB];
     float rx[4], rz[4], nx[4], nz[4];               // x, z of the tile being walked and of the next
-    const auto frame = [&](int s) -> long long {    // clamped: what is read behind the row is thrown away below
-        s = min(s, q.len - 1);
-        return p.reverse ? q.len - 1 - s : s;
+    const unsigned off = d * (unsigned)sizeof(TY);
+    const auto fetch = [&](int tile, auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const int s0 = tile * TS + w * 4;
+        fetch_rows<FULL>(lx, px, p.x_st, s0, q.len, p.reverse, off);
+        fetch_rows<FULL>(ldt, pdt, p.dt_st, s0, q.len, p.reverse, off);
+        if (!PRE && pz) fetch_rows<FULL>(lz, pz, p.z_st, s0, q.len, p.reverse, off);
+        fetch_states<TY, NP, RB>(lB, pB, p.b_st, tile, q.len, p.reverse, p.N);
+        if (!PRE) fetch_states<TY, NP, RB>(lC, pC, p.c_st, tile, q.len, p.reverse, p.N);
     };
-    const auto fetch = [&](int tile) {
+    const auto place = [&](int tile, int half, auto full) {
+        constexpr bool FULL = decltype(full)::value;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const long long f = frame(tile * TS + w * 4 + i);
-            lx[i] = (px + f * p.x_st)[d];
-            ldt[i] = (pdt + f * p.dt_st)[d];
-            if (!PRE && pz) lz[i] = (pz + f * p.z_st)[d];
-        }
-#pragma unroll
-        for (int k = 0; k < RB; ++k) {
-            const int e = tid + k * 256;
-            const long long f = frame(tile * TS + e / NP);
-            const int n = min(e % NP, p.N - 1);
-            if (RB * 256 == TS * NP || e < TS * NP) {
-                lB[k] = (pB + f * p.b_st)[n];
-                if (!PRE) lC[k] = (pC + f * p.c_st)[n];
-            }
-        }
-    };
-    const auto place = [&](int tile, int half) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool ok = tile * TS + w * 4 + i < q.len;
+            const bool ok = FULL || tile * TS + w * 4 + i < q.len;
             const float v = (float)ldt[i] + bias;
-            const float de = ok ? (p.softplus ? softplus_(v) : v) : 0.f;
+            const float sp = p.softplus ? softplus_(v) : v;
+            const float de = ok ? sp : 0.f;
             nx[i] = ok ? (float)lx[i] : 0.f;
-            nz[i] = (!PRE && pz && ok) ? (float)lz[i] : 0.f;
+            nz[i] = (!PRE && pz) ? (float)lz[i] : 0.f;
             s_du[half][w * 4 + i][lane] = float2{de, de * nx[i]};
         }
-#pragma unroll
-        for (int k = 0; k < RB; ++k) {
-            const int e = tid + k * 256;
-            if (RB * 256 == TS * NP || e < TS * NP) {
-                const bool ok = tile * TS + e / NP < q.len && e % NP < p.N;
-                s_B[half][e] = ok ? (float)lB[k] : 0.f;
-                if (!PRE) s_C[half][e] = ok ? (float)lC[k] : 0.f;
-            }
-        }
+        place_states<TY, NP, RB>(s_B[half], lB, tile, q.len, p.N);
+        if (!PRE) place_states<TY, NP, RB>(s_C[half], lC, tile, q.len, p.N);
     };
-    if (q.t0 < q.t1) {
-        fetch(q.t0);
-        place(q.t0, 0);
-        fetch(min(q.t0 + 1, q.t1 - 1));
-        __syncthreads();
-    }
-    for (int tile = q.t0; tile < q.t1; ++tile) {
-        const int half = (tile - q.t0) & 1, sb = tile * TS;
+    float* ck = (!PRE && p.ckpt) ? p.ckpt + (((size_t)q.t0 * p.B + q.b) * NP + w * SPL) * p.D : nullptr;
+    const size_t ck_tile = (size_t)p.B * NP * p.D;
+    // a tile; FULL: it, the next and the one after that hold valid frames alone
+    const auto walk = [&](int tile, auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const int half = (tile - q.t0) & 1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) { rx[i] = nx[i]; rz[i] = nz[i]; }
-        if (!PRE && p.ckpt && q.on) {
-            float* ck = p.ckpt + (((size_t)tile * p.B + q.b) * NP + w * SPL) * p.D;
+        if (!PRE && ck) {
+            if (q.on)
 #pragma unroll
-            for (int m = 0; m < NB; ++m)
+                for (int m = 0; m < NB; ++m)
 #pragma unroll
-                for (int j = 0; j < SPL; ++j) (ck + (size_t)(m * 4 * SPL + j) * p.D)[d] = h[m][j];
+                    for (int j = 0; j < SPL; ++j)
+                        *(float*)((char*)(ck + (size_t)(m * 4 * SPL + j) * p.D) + d * 4u) = h[m][j];
+            ck += ck_tile;
         }
 #pragma unroll
         for (int t = 0; t < TS; ++t) {
@@ -124,25 +107,33 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
             if (!PRE) s_y[half][w][t][lane] = y;
             else if (w == 0) dsum += du.x;
         }
-        if (tile + 1 < q.t1) {
-            place(tile + 1, half ^ 1);
-            fetch(min(tile + 2, q.t1 - 1));
+        if (FULL || tile + 1 < q.t1) {
+            place(tile + 1, half ^ 1, full);
+            fetch(FULL ? tile + 2 : min(tile + 2, q.t1 - 1), full);
         }
         __syncthreads();
         if (!PRE && q.on) {
+            float y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int t = w * 4 + i, s = sb + t;
-                if (s >= p.T) continue;
-                float y = ((s_y[half][0][t][lane] + s_y[half][1][t][lane]) +
-                           (s_y[half][2][t][lane] + s_y[half][3][t][lane])) + Dk * rx[i];
-                if (pz) y *= silu_(rz[i]);
-                const bool ok = s < q.len;
-                const long long f = (p.reverse && ok) ? q.len - 1 - s : s;
-                (po + f * p.o_st)[d] = (TY)(ok ? y : 0.f);
+                const int t = w * 4 + i;
+                y[i] = ((s_y[half][0][t][lane] + s_y[half][1][t][lane]) +
+                        (s_y[half][2][t][lane] + s_y[half][3][t][lane])) + Dk * rx[i];
+                if (pz) y[i] *= silu_(rz[i]);
             }
+            store_rows<FULL>(po, p.o_st, tile * TS + w * 4, q.len, p.T, p.reverse, off, y);
         }
+    };
+    if (q.t0 < q.t1) {
+        fetch(q.t0, Flag<false>{});
+        place(q.t0, 0, Flag<false>{});
+        fetch(min(q.t0 + 1, q.t1 - 1), Flag<false>{});
+        __syncthreads();
     }
+    const int clear = min(q.t1, q.len / TS) - 2;
+    int tile = q.t0;
+    for (; tile < clear; ++tile) walk(tile, Flag<true>{});
+    for (; tile < q.t1; ++tile) walk(tile, Flag<false>{});
     if (!q.on) return;
     if (PRE) {
 #pragma unroll
