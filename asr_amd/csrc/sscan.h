@@ -79,7 +79,10 @@ __device__ __forceinline__ void fetch_rows(TY (&o)[4], const TY* base, long long
         const char* r = b + (long long)(reverse ? len - 1 - s0 : s0) * sb;
         const long long step = reverse ? -sb : sb;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { o[i] = *(const TY*)(r + off); r += step; }
+        for (int i = 0; i < 4; ++i) {
+            o[i] = *(const TY*)(r + off);
+            r += step;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -98,7 +101,10 @@ __device__ __forceinline__ void store_rows(TY* base, long long st, int s0, int l
         char* r = b + (long long)(reverse ? len - 1 - s0 : s0) * sb;
         const long long step = reverse ? -sb : sb;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { *(TY*)(r + off) = (TY)v[i]; r += step; }
+        for (int i = 0; i < 4; ++i) {
+            *(TY*)(r + off) = (TY)v[i];
+            r += step;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -126,5 +132,13 @@ __device__ __forceinline__ void place_states(float* dst, const TY (&o)[RB], int 
         if (RB * 256 == SSCAN_TS * NP || e < SSCAN_TS * NP)
             dst[e] = (tile * SSCAN_TS + e / NP < len && e % NP < N) ? (float)o[k] : 0.f;
     }
+}
+// The kernel's arguments, read again where they are used: kept in scalar registers over the whole loop they do not fit, and
+// the compiler moves them through vector registers, lane by lane.
+typedef const __attribute__((address_space(4))) SscanArgs* KArgs;
+__device__ __forceinline__ KArgs kargs() {
+    KArgs k = (KArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(k));
+    return k;
 }
 template <bool V> struct Flag { static constexpr bool value = V; };

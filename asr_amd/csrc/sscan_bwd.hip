@@ -36,47 +36,46 @@ __device__ __forceinline__ float sum16(const float (&v)[16], int lane) {
 }
 
 // PRE: the adjoint a chunk hands to the one in front of it when nothing comes in from behind, and its sum of delta.
+// Half way through a tile's adjoints, when half of its states have left their registers, the tile in front of it is called from
+// memory; it goes into the other half of the input buffers behind the last adjoint.  (Called a tile earlier, as the forward
+// pass does, it costs 30 registers where they are scarcest: one wave per SIMD less, or spills.)
 template <typename TY, int SPL, int NB, bool PRE>
-__global__ __launch_bounds__(256) void sstate_bwd_kernel(SscanArgs p) {
+__global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanArgs p) {
     constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RS = 8 / SPL;    // RS frames give sixteen sums
-    __shared__ float2 s_du[TS][64];
-    __shared__ float s_dy[TS][64];
-    __shared__ __attribute__((aligned(16))) float s_B[PRE ? 1 : TS][NP], s_C[TS][NP];
+    constexpr int RB = (TS * NP + 255) / 256;
+    __shared__ float2 s_du[2][TS][64];
+    __shared__ float s_dy[2][TS][64];
+    __shared__ __attribute__((aligned(16))) float s_B[2][PRE ? 1 : TS * NP], s_C[2][TS * NP];
     __shared__ float2 s_s[PRE ? 1 : 4][PRE ? 1 : TS][64];
     __shared__ float s_y[PRE ? 1 : 4][PRE ? 1 : TS][64];
-    __shared__ float s_bc[PRE ? 1 : TS][2][NP];
+    __shared__ float s_bc[PRE ? 1 : TS * 2 * NP];
     const Place q = sscan_place(p);
     const int tid = threadIdx.x, lane = q.lane, w = q.w;
     if (PRE && (q.k == 0 || q.t0 >= q.t1)) return;
-    const TY* px = (const TY*)p.x + q.b * p.x_sb + q.d;
-    const TY* pdt = (const TY*)p.dt + q.b * p.dt_sb + q.d;
-    const TY* pz = p.z ? (const TY*)p.z + q.b * p.z_sb + q.d : nullptr;
-    const TY* pdo = (const TY*)p.dout + q.b * p.do_sb + q.d;
-    const TY* pB = (const TY*)p.Bm + q.b * p.b_sb + q.g * p.b_sg;
-    const TY* pC = (const TY*)p.Cm + q.b * p.c_sb + q.g * p.c_sg;
-    const size_t obase = (size_t)q.b * p.D + q.d, ostep = (size_t)p.B * p.D;
-    const float bias = p.bias ? p.bias[q.d] : 0.f;
-    const float Dk = p.Dk ? p.Dk[q.d] : 0.f;
+    const bool gated = p.z != nullptr, soft = p.softplus;
+    const unsigned d = q.d, off = d * (unsigned)sizeof(TY);
+    const float bias = p.bias ? p.bias[d] : 0.f;
+    const float Dk = p.Dk ? p.Dk[d] : 0.f;
     float A2[NB][SPL], r[NB][SPL], dA[NB][SPL];
 #pragma unroll
     for (int m = 0; m < NB; ++m)
 #pragma unroll
         for (int j = 0; j < SPL; ++j) {
             const int n = (m * 4 + w) * SPL + j;
-            A2[m][j] = n < p.N ? p.A[(size_t)q.d * p.N + n] * LOG2E : 0.f;
-            r[m][j] = (!PRE && p.dh_last && n < p.N) ? p.dh_last[((size_t)q.b * p.D + q.d) * p.N + n] : 0.f;
+            A2[m][j] = n < p.N ? p.A[(size_t)d * p.N + n] * LOG2E : 0.f;
+            r[m][j] = (!PRE && p.dh_last && n < p.N) ? p.dh_last[((size_t)q.b * p.D + d) * p.N + n] : 0.f;
             dA[m][j] = 0.f;
         }
     const int nch = (q.nt + p.tpc - 1) / p.tpc;                       // chunks that hold a valid frame
     if (!PRE) {                                                       // the adjoint that comes in from behind
         for (int j = nch - 1; j > q.k; --j) {
-            const float ds = p.c_ds[((size_t)j * p.B + q.b) * p.D + q.d];
+            const float ds = p.c_ds[((size_t)j * p.B + q.b) * p.D + d];
 #pragma unroll
             for (int m = 0; m < NB; ++m)
 #pragma unroll
                 for (int i = 0; i < SPL; ++i) {
                     const int n = (m * 4 + w) * SPL + i;
-                    const float rl = p.c_h[(((size_t)j * p.B + q.b) * NP + n) * p.D + q.d];
+                    const float rl = p.c_h[(((size_t)j * p.B + q.b) * NP + n) * p.D + d];
                     r[m][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][i] * ds), r[m][i], rl);
                 }
         }
@@ -88,148 +87,211 @@ __global__ __launch_bounds__(256) void sstate_bwd_kernel(SscanArgs p) {
             for (int j = 0; j < SPL; ++j) r[m][j] = 0.f;
     }
     float accD = 0.f, accb = 0.f, dsum = 0.f;
-    for (int tile = q.t1 - 1; tile >= q.t0; --tile) {
-        const int sb = tile * TS;
-        float rx[4], rz[4], rg[4], rr[4], rd[4], ry[4];              // own frames: x, z, dout, dt + bias, delta, dy
+    TY lx[4], ldt[4], lz[4], lg[4], lB[RB], lC[RB];       // on their way from memory
+    float rx[4], rs[4], rg[4], nx[4], ns[4], ng[4];       // x, d delta / d dt, dout silu'(z): of the tile walked and the next
+    const auto fetch = [&](int tile, auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const KArgs k = kargs();
+        const int s0 = tile * TS + w * 4, rev = k->reverse;
+        if (!PRE) fetch_rows<FULL>(lx, (const TY*)k->x + q.b * k->x_sb, k->x_st, s0, q.len, rev, off);
+        fetch_rows<FULL>(ldt, (const TY*)k->dt + q.b * k->dt_sb, k->dt_st, s0, q.len, rev, off);
+        fetch_rows<FULL>(lg, (const TY*)k->dout + q.b * k->do_sb, k->do_st, s0, q.len, rev, off);
+        if (gated) fetch_rows<FULL>(lz, (const TY*)k->z + q.b * k->z_sb, k->z_st, s0, q.len, rev, off);
+        if (!PRE) fetch_states<TY, NP, RB>(lB, (const TY*)k->Bm + q.b * k->b_sb + q.g * k->b_sg, k->b_st, tile, q.len, rev, k->N);
+        fetch_states<TY, NP, RB>(lC, (const TY*)k->Cm + q.b * k->c_sb + q.g * k->c_sg, k->c_st, tile, q.len, rev, k->N);
+    };
+    const auto place = [&](int tile, int half, auto full) {
+        constexpr bool FULL = decltype(full)::value;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = sb + w * 4 + i;
-            rx[i] = rz[i] = rg[i] = rr[i] = rd[i] = ry[i] = 0.f;
-            if (s < q.len) {
-                const long long f = p.reverse ? q.len - 1 - s : s;
-                rx[i] = ldf(px + f * p.x_st);
-                rr[i] = ldf(pdt + f * p.dt_st) + bias;
-                rg[i] = ldf(pdo + f * p.do_st);
-                if (pz) rz[i] = ldf(pz + f * p.z_st);
-                rd[i] = p.softplus ? softplus_(rr[i]) : rr[i];
-                ry[i] = pz ? rg[i] * silu_(rz[i]) : rg[i];
+            const bool ok = FULL || tile * TS + w * 4 + i < q.len;
+            const float v = (float)ldt[i] + bias, g = ok ? (float)lg[i] : 0.f;
+            float de = v, dy = g;
+            ns[i] = 1.f;
+            if (soft) {
+                const float u = exp_neg_abs_(v);
+                de = softplus_from_(v, u);
+                ns[i] = sigmoid_from_(v, u);
             }
-            s_du[w * 4 + i][lane] = float2{rd[i], q.on ? rd[i] * rx[i] : 0.f};
-            s_dy[w * 4 + i][lane] = q.on ? ry[i] : 0.f;
-        }
-        for (int i = tid; i < TS * NP; i += 256) {
-            const int st = i / NP, n = i % NP, s = sb + st;
-            float vb = 0.f, vc = 0.f;
-            if (s < q.len && n < p.N) {
-                const long long f = p.reverse ? q.len - 1 - s : s;
-                if (!PRE) vb = ldf(pB + f * p.b_st + n);
-                vc = ldf(pC + f * p.c_st + n);
+            if (!ok) de = ns[i] = 0.f;
+            if (gated) {
+                const float z = ok ? (float)lz[i] : 0.f, sg = sigm_(z);
+                dy = g * z * sg;
+                ng[i] = g * dsilu_(z, sg);
             }
-            if (!PRE) s_B[st][n] = vb;
-            s_C[st][n] = vc;
+            nx[i] = (PRE || !ok) ? 0.f : (float)lx[i];
+            s_du[half][w * 4 + i][lane] = float2{de, q.on ? de * nx[i] : 0.f};
+            s_dy[half][w * 4 + i][lane] = q.on ? dy : 0.f;
         }
-        __syncthreads();
+        const int N = kargs()->N;
+        if (!PRE) place_states<TY, NP, RB>(s_B[half], lB, tile, q.len, N);
+        place_states<TY, NP, RB>(s_C[half], lC, tile, q.len, N);
+    };
+    // the state in front of a tile, first group of states: fetched a tile ahead
+    float hn[SPL];
+    const auto state = [&](int tile, int m, float (&o)[SPL]) {
+        const KArgs k = kargs();
+        const char* ck = (const char*)(k->ckpt + (((size_t)tile * k->B + q.b) * NP + (m * 4 + w) * SPL) * k->D);
+        unsigned at = d * 4u;
+#pragma unroll
+        for (int j = 0; j < SPL; ++j) {
+            o[j] = *(const float*)(ck + at);
+            ck += (size_t)k->D * 4;
+        }
+    };
+    // a tile; FULL: it and the one in front of it hold valid frames alone, and that is this chunk's too
+    const auto walk = [&](int tile, auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const int half = (q.t1 - 1 - tile) & 1, sb = tile * TS;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { rx[i] = nx[i]; rs[i] = ns[i]; rg[i] = ng[i]; }
         if (PRE) {
-#pragma unroll 4
+            if (FULL || tile > q.t0) fetch(tile - 1, full);
+#pragma unroll
             for (int t = TS - 1; t >= 0; --t) {
-                const float de = s_du[t][lane].x, dy = s_dy[t][lane];
+                const float de = s_du[half][t][lane].x, dy = s_dy[half][t][lane];
 #pragma unroll
                 for (int m = 0; m < NB; ++m)
 #pragma unroll
                     for (int j = 0; j < SPL; ++j)
-                        r[m][j] = __builtin_amdgcn_exp2f(A2[m][j] * de) * __builtin_fmaf(s_C[t][(m * 4 + w) * SPL + j], dy, r[m][j]);
+                        r[m][j] = __builtin_amdgcn_exp2f(A2[m][j] * de) *
+                                  __builtin_fmaf(s_C[half][t * NP + (m * 4 + w) * SPL + j], dy, r[m][j]);
                 if (w == 0) dsum += de;
             }
-            __syncthreads();
-            continue;
-        }
-        const float* ck = p.ckpt + ((size_t)tile * p.B + q.b) * NP * p.D + q.d;
+        } else {
 #pragma unroll
-        for (int m = 0; m < NB; ++m) {
-            float a[TS][SPL], h[TS][SPL], h0[SPL], da[SPL];    // da: a tile's part of dA, so that no sum runs over all frames
+            for (int m = 0; m < NB; ++m) {
+                float a[TS][SPL], h[TS][SPL], h0[SPL], da[SPL];    // da: a tile's part of dA: no sum runs over all frames
+                if (m == 0) {
 #pragma unroll
-            for (int j = 0; j < SPL; ++j) da[j] = 0.f;
-#pragma unroll
-            for (int j = 0; j < SPL; ++j) h0[j] = ck[(size_t)((m * 4 + w) * SPL + j) * p.D];
-#pragma unroll
-            for (int t = 0; t < TS; ++t) {
-                const float2 du = s_du[t][lane];
-                float y = 0.f;
-#pragma unroll
-                for (int j = 0; j < SPL; ++j) {
-                    const int n = (m * 4 + w) * SPL + j;
-                    a[t][j] = __builtin_amdgcn_exp2f(A2[m][j] * du.x);
-                    h[t][j] = __builtin_fmaf(a[t][j], t ? h[t - 1][j] : h0[j], du.y * s_B[t][n]);
-                    y = __builtin_fmaf(s_C[t][n], h[t][j], y);
+                    for (int j = 0; j < SPL; ++j) h0[j] = hn[j];
+                } else {
+                    state(tile, m, h0);
                 }
-                if (pz) { if (m) s_y[w][t][lane] += y; else s_y[w][t][lane] = y; }
-            }
 #pragma unroll
-            for (int tb = TS / RS - 1; tb >= 0; --tb) {
-                float v[16];
+                for (int j = 0; j < SPL; ++j) da[j] = 0.f;
 #pragma unroll
-                for (int i = RS - 1; i >= 0; --i) {
-                    const int t = tb * RS + i;
-                    const float2 du = s_du[t][lane];
-                    const float dy = s_dy[t][lane];
-                    float s1 = 0.f, s2 = 0.f;
+                for (int t = 0; t < TS; ++t) {
+                    const float2 du = s_du[half][t][lane];
+                    float y = 0.f;
 #pragma unroll
                     for (int j = 0; j < SPL; ++j) {
-                        const int n = (m * 4 + w) * SPL + j;
-                        const float dh = __builtin_fmaf(s_C[t][n], dy, r[m][j]);
-                        v[i * 2 * SPL + j] = dh * du.y;
-                        v[i * 2 * SPL + SPL + j] = dy * h[t][j];
-                        r[m][j] = a[t][j] * dh;
-                        const float qq = r[m][j] * (t ? h[t - 1][j] : h0[j]);
-                        s2 = __builtin_fmaf(qq, A2[m][j], s2);
-                        da[j] = __builtin_fmaf(qq, du.x, da[j]);
-                        s1 = __builtin_fmaf(dh, s_B[t][n], s1);
+                        const int e = t * NP + (m * 4 + w) * SPL + j;
+                        a[t][j] = __builtin_amdgcn_exp2f(A2[m][j] * du.x);
+                        h[t][j] = __builtin_fmaf(a[t][j], t ? h[t - 1][j] : h0[j], du.y * s_B[half][e]);
+                        y = __builtin_fmaf(s_C[half][e], h[t][j], y);
                     }
-                    if (m) { s_s[w][t][lane].x += s1; s_s[w][t][lane].y += s2; }
-                    else s_s[w][t][lane] = float2{s1, s2};
+                    if (gated) { if (m) s_y[w][t][lane] += y; else s_y[w][t][lane] = y; }
                 }
-                const float z = sum16(v, lane);
-                if ((lane & 3) == 0) {
-                    const int id = lane >> 2, t = tb * RS + id / (2 * SPL), c = (id / SPL) & 1, j = id % SPL;
-                    s_bc[t][c][(m * 4 + w) * SPL + j] = z;
-                }
-            }
 #pragma unroll
-            for (int j = 0; j < SPL; ++j) dA[m][j] += da[j];
+                for (int tb = TS / RS - 1; tb >= 0; --tb) {
+                    float v[16];
+#pragma unroll
+                    for (int i = RS - 1; i >= 0; --i) {
+                        const int t = tb * RS + i;
+                        const float2 du = s_du[half][t][lane];
+                        const float dy = s_dy[half][t][lane];
+                        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+                        for (int j = 0; j < SPL; ++j) {
+                            const int e = t * NP + (m * 4 + w) * SPL + j;
+                            const float dh = __builtin_fmaf(s_C[half][e], dy, r[m][j]);
+                            v[i * 2 * SPL + j] = dh * du.y;
+                            v[i * 2 * SPL + SPL + j] = dy * h[t][j];
+                            r[m][j] = a[t][j] * dh;
+                            const float qq = r[m][j] * (t ? h[t - 1][j] : h0[j]);
+                            s2 = __builtin_fmaf(qq, A2[m][j], s2);
+                            da[j] = __builtin_fmaf(qq, du.x, da[j]);
+                            s1 = __builtin_fmaf(dh, s_B[half][e], s1);
+                        }
+                        if (m) { s_s[w][t][lane].x += s1; s_s[w][t][lane].y += s2; }
+                        else s_s[w][t][lane] = float2{s1, s2};
+                    }
+                    if (m == NB - 1 && tb == TS / RS / 2 && (FULL || tile > q.t0)) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        fetch(tile - 1, full);
+                        state(tile - 1, 0, hn);
+                    }
+                    const float z = sum16(v, lane);
+                    if ((lane & 3) == 0) {
+                        const int id = lane >> 2, t = tb * RS + id / (2 * SPL), c = (id / SPL) & 1, j = id % SPL;
+                        s_bc[(t * 2 + c) * NP + (m * 4 + w) * SPL + j] = z;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < SPL; ++j) dA[m][j] += da[j];
+            }
+        }
+        // this tile's delta, delta x and dy of the own frames, before their buffers are written again
+        float de[4], dy[4];
+        if (!PRE) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { de[i] = s_du[half][w * 4 + i][lane].x; dy[i] = s_dy[half][w * 4 + i][lane]; }
+        }
+        if (FULL || tile > q.t0) {
+            place(tile - 1, half ^ 1, full);
         }
         __syncthreads();
+        if (PRE) return;
+        const int s0 = sb + w * 4;
+        float ox[4], odt[4], oz[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int t = w * 4 + i, s = sb + t;
-            if (s >= p.T || !q.on) continue;
-            const float s1 = (s_s[0][t][lane].x + s_s[1][t][lane].x) + (s_s[2][t][lane].x + s_s[3][t][lane].x);
-            const float s2 = (s_s[0][t][lane].y + s_s[1][t][lane].y) + (s_s[2][t][lane].y + s_s[3][t][lane].y);
-            const bool ok = s < q.len;
-            const long long f = (p.reverse && ok) ? q.len - 1 - s : s;
-            const size_t o = f * ostep + obase;
-            float ddt = __builtin_fmaf(rx[i], s1, s2 * LN2);
-            if (p.softplus) ddt *= sigm_(rr[i]);
-            stf((TY*)p.dx + o, ok ? __builtin_fmaf(rd[i], s1, Dk * ry[i]) : 0.f);
-            stf((TY*)p.ddt + o, ok ? ddt : 0.f);
-            if (pz) {
-                const float y = ((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i];
-                stf((TY*)p.dz + o, ok ? rg[i] * y * dsilu_(rz[i], sigm_(rz[i])) : 0.f);
-            }
-            if (ok) { accD = __builtin_fmaf(ry[i], rx[i], accD); accb += ddt; }
+            const int t = w * 4 + i;
+            const float2 a = s_s[0][t][lane], b = s_s[1][t][lane], c = s_s[2][t][lane], e = s_s[3][t][lane];
+            const float s1 = (a.x + b.x) + (c.x + e.x), s2 = (a.y + b.y) + (c.y + e.y);
+            ox[i] = __builtin_fmaf(de[i], s1, Dk * dy[i]);
+            odt[i] = __builtin_fmaf(rx[i], s1, s2 * LN2) * rs[i];
+            if (gated) oz[i] = rg[i] * (((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i]);
+            accD = __builtin_fmaf(dy[i], rx[i], accD);     // frames of the padding give zeros
+            accb += odt[i];
         }
-        float* pbc = p.part_bc + (((size_t)(q.g * p.tpg + q.ct) * p.B + q.b) * p.T + sb) * (2 * NP);
-        for (int i = tid; i < TS * 2 * NP; i += 256)
-            if (sb + i / (2 * NP) < q.len) pbc[i] = s_bc[i / (2 * NP)][(i / NP) & 1][i % NP];
+        const KArgs k = kargs();
+        const int T = k->T, rev = k->reverse;
+        const long long ost = (long long)k->B * k->D, orow = (long long)q.b * k->D;
+        if (q.on) {
+            store_rows<FULL>((TY*)k->dx + orow, ost, s0, q.len, T, rev, off, ox);
+            store_rows<FULL>((TY*)k->ddt + orow, ost, s0, q.len, T, rev, off, odt);
+            if (gated) store_rows<FULL>((TY*)k->dz + orow, ost, s0, q.len, T, rev, off, oz);
+        }
+        char* pbc = (char*)(k->part_bc + (((size_t)(q.g * k->tpg + q.ct) * k->B + q.b) * T + sb) * (2 * NP));
+        unsigned first = tid;
+#pragma unroll
+        for (int i = 0; i < (TS * 2 * NP + 255) / 256; ++i) {
+            const unsigned e = first + i * 256;
+            if ((TS * 2 * NP % 256 == 0 || e < TS * 2 * NP) && (FULL || sb + (int)(e / (2 * NP)) < q.len))
+                *(float*)(pbc + e * 4u) = s_bc[e];
+        }
+        __syncthreads();
+    };
+    if (q.t0 < q.t1) {
+        fetch(q.t1 - 1, Flag<false>{});
+        if (!PRE) state(q.t1 - 1, 0, hn);
+        place(q.t1 - 1, 0, Flag<false>{});
         __syncthreads();
     }
+    int tile = q.t1 - 1;
+    for (; tile >= q.t0 && (tile * TS + TS > q.len); --tile) walk(tile, Flag<false>{});
+    for (; tile >= q.t0 + 1; --tile) walk(tile, Flag<true>{});
+    for (; tile >= q.t0; --tile) walk(tile, Flag<false>{});
     if (PRE) {
         if (!q.on) return;
 #pragma unroll
         for (int m = 0; m < NB; ++m)
 #pragma unroll
             for (int j = 0; j < SPL; ++j)
-                p.c_h[(((size_t)q.k * p.B + q.b) * NP + (m * 4 + w) * SPL + j) * p.D + q.d] = r[m][j];
-        if (w == 0) p.c_ds[((size_t)q.k * p.B + q.b) * p.D + q.d] = dsum;
+                p.c_h[(((size_t)q.k * p.B + q.b) * NP + (m * 4 + w) * SPL + j) * p.D + d] = r[m][j];
+        if (w == 0) p.c_ds[((size_t)q.k * p.B + q.b) * p.D + d] = dsum;
         return;
     }
     // padding, the parts of the parameter gradients, the gradient of the first state
     const int send = min(p.T, (q.t0 + p.tpc) * TS);
     if (q.on) {
         for (int s = max(q.nt, q.t0) * TS + w; s < send; s += 4) {
-            const size_t o = s * ostep + obase;
+            const size_t o = ((size_t)s * p.B + q.b) * p.D + d;
             stf((TY*)p.dx + o, 0.f);
             stf((TY*)p.ddt + o, 0.f);
-            if (pz) stf((TY*)p.dz + o, 0.f);
+            if (gated) stf((TY*)p.dz + o, 0.f);
         }
     }
     const size_t row = (size_t)q.k * p.B + q.b;
@@ -240,17 +302,17 @@ __global__ __launch_bounds__(256) void sstate_bwd_kernel(SscanArgs p) {
             for (int j = 0; j < SPL; ++j) {
                 const int n = (m * 4 + w) * SPL + j;
                 if (n >= p.N) continue;
-                p.part_a[(row * p.D + q.d) * p.N + n] = dA[m][j];
-                if (p.dh0 && q.k == 0) p.dh0[((size_t)q.b * p.D + q.d) * p.N + n] = r[m][j];
+                p.part_a[(row * p.D + d) * p.N + n] = dA[m][j];
+                if (p.dh0 && q.k == 0) p.dh0[((size_t)q.b * p.D + d) * p.N + n] = r[m][j];
             }
     }
     __syncthreads();
-    s_dy[w][lane] = accD;
-    s_dy[4 + w][lane] = accb;
+    s_dy[0][w][lane] = accD;
+    s_dy[0][4 + w][lane] = accb;
     __syncthreads();
     if (w < 2 && q.on) {
-        const float t = (s_dy[w * 4][lane] + s_dy[w * 4 + 1][lane]) + (s_dy[w * 4 + 2][lane] + s_dy[w * 4 + 3][lane]);
-        (w ? p.part_b : p.part_d)[row * p.D + q.d] = t;
+        const float* v = &s_dy[0][w * 4][lane];
+        (w ? p.part_b : p.part_d)[row * p.D + d] = (v[0] + v[64]) + (v[128] + v[192]);
     }
 }
 

@@ -84,12 +84,15 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { rx[i] = nx[i]; rz[i] = nz[i]; }
         if (!PRE && ck) {
+            unsigned at = d * 4u;
             if (q.on)
 #pragma unroll
                 for (int m = 0; m < NB; ++m)
 #pragma unroll
-                    for (int j = 0; j < SPL; ++j)
-                        *(float*)((char*)(ck + (size_t)(m * 4 * SPL + j) * p.D) + d * 4u) = h[m][j];
+                    for (int j = 0; j < SPL; ++j) {
+                        char* r = (char*)(ck + (size_t)(m * 4 * SPL + j) * p.D);
+                        *(float*)(r + at) = h[m][j];
+                    }
             ck += ck_tile;
         }
 #pragma unroll
