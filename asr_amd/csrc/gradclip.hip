@@ -27,22 +27,22 @@ __device__ __forceinline__ int find_tensor(const ClipList& l, int chunk) {
     return lo;
 }
 
+// 16 bytes at a time at any address that suits T: the results of one type lie behind one another in one buffer.
+template <typename T> struct Any16 {
+    typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+
 template <typename T>
 __device__ __forceinline__ double chunk_sq(const T* p, int n) {
     constexpr int V = 16 / sizeof(T);
     double acc = 0.0;
-    int i0 = 0;
-    if (((uintptr_t)p & 15) == 0) {
-        const int nv = n / V;
-        for (int i = threadIdx.x; i < nv; i += 256) {
-            float v[V];
-            ldv<T, V>(p + i * V, v);
+    const int nv = n / V;
+    for (int i = threadIdx.x; i < nv; i += 256) {
+        const typename Any16<T>::type v = *(const typename Any16<T>::type*)(p + i * V);
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc = __builtin_fma((double)v[e], (double)v[e], acc);
-        }
-        i0 = nv * V;
+        for (int e = 0; e < V; ++e) acc = __builtin_fma((double)(float)v[e], (double)(float)v[e], acc);
     }
-    for (int i = i0 + threadIdx.x; i < n; i += 256) {
+    for (int i = nv * V + threadIdx.x; i < n; i += 256) {
         const double v = (double)ldf(p + i);
         acc = __builtin_fma(v, v, acc);
     }
@@ -86,19 +86,14 @@ __global__ __launch_bounds__(1024) void clip_norm_kernel(const double* __restric
 template <typename T>
 __device__ __forceinline__ void chunk_scale(const T* p, T* q, int n, float m) {
     constexpr int V = 16 / sizeof(T);
-    int i0 = 0;
-    if ((((uintptr_t)p | (uintptr_t)q) & 15) == 0) {
-        const int nv = n / V;
-        for (int i = threadIdx.x; i < nv; i += 256) {
-            float v[V];
-            ldv<T, V>(p + i * V, v);
+    const int nv = n / V;
+    for (int i = threadIdx.x; i < nv; i += 256) {
+        typename Any16<T>::type v = *(const typename Any16<T>::type*)(p + i * V);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] *= m;
-            stv<T, V>(q + i * V, v);
-        }
-        i0 = nv * V;
+        for (int e = 0; e < V; ++e) v[e] = (T)((float)v[e] * m);
+        *(typename Any16<T>::type*)(q + i * V) = v;
     }
-    for (int i = i0 + threadIdx.x; i < n; i += 256) stf(q + i, ldf(p + i) * m);
+    for (int i = nv * V + threadIdx.x; i < n; i += 256) stf(q + i, ldf(p + i) * m);
 }
 
 __global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const float* __restrict__ mult) {

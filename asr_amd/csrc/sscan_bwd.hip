@@ -316,30 +316,60 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
     }
 }
 
-// dB / dC: the parts of a group's channel tiles added in order, written in the activation type at the frame's place
+// The sums over workgroups, one launch.  Blocks [0, nbc * G): dB / dC, the parts of a group's channel tiles added in order and
+// written in the activation type at the frame's place.  Behind them, 64 columns a block: dA, dD and d dt_bias, the parts of
+// all rows and chunks (P of them) added by four groups of lanes and joined in order.
 template <typename TY>
-__global__ __launch_bounds__(256) void sscan_dbc_kernel(const float* __restrict__ part, int T, int B, int N, int NP, int G,
-                                                        int tpg, int reverse, const int* __restrict__ lens, TY* dB, TY* dC) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const size_t per = (size_t)B * T * 2 * NP;
-    if (i >= per) return;
-    const int g = blockIdx.y;
-    const int n = (int)(i % NP), c = (int)(i / NP) & 1;
-    const size_t bs = i / (2 * NP);
-    const int b = (int)(bs / T), s = (int)(bs % T);
-    if (n >= N) return;
-    const int len = row_len(lens, b, T);
+__global__ __launch_bounds__(256) void sscan_finish_kernel(SscanArgs p, TY* dB, TY* dC, float* dA, float* dD, float* db,
+                                                           unsigned nbc, unsigned na, unsigned nd) {
+    __shared__ float sm[4][64];
+    unsigned blk = blockIdx.x;
+    if (blk < nbc * p.G) {
+        const int g = blk / nbc;
+        const size_t i = (size_t)(blk % nbc) * 256 + threadIdx.x, per = (size_t)p.B * p.T * 2 * p.np;
+        if (i >= per) return;
+        const int n = (int)(i % p.np), c = (int)(i / p.np) & 1;
+        const size_t bs = i / (2 * p.np);
+        const int b = (int)(bs / p.T), s = (int)(bs % p.T);
+        if (n >= p.N) return;
+        const int len = row_len(p.lens, b, p.T);
+        float v = 0.f;
+        if (s < len) {
+            const float* q = p.part_bc + (size_t)g * p.tpg * per + i;
+#pragma unroll 8
+            for (int k = 0; k < p.tpg; ++k) v += q[(size_t)k * per];
+        }
+        const long long f = (p.reverse && s < len) ? len - 1 - s : s;
+        stf((c ? dC : dB) + ((f * p.B + b) * p.G + g) * p.N + n, v);
+        return;
+    }
+    blk -= nbc * p.G;
+    const float* part = p.part_a;
+    float* out = dA;
+    size_t n = (size_t)p.D * p.N;
+    if (blk >= na) {                                  // dD's blocks, if it is wanted, then d dt_bias's
+        blk -= na;
+        n = p.D;
+        const bool second = !dD || blk >= nd;
+        if (dD && second) blk -= nd;
+        part = second ? p.part_b : p.part_d;
+        out = second ? db : dD;
+    }
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, P = p.S * p.B;
+    const size_t i = (size_t)blk * 64 + lane;
     float v = 0.f;
-    if (s < len)
-        for (int k = 0; k < tpg; ++k) v += part[((size_t)g * tpg + k) * per + i];
-    const long long f = (reverse && s < len) ? len - 1 - s : s;
-    stf((c ? dC : dB) + ((f * B + b) * G + g) * N + n, v);
+    if (i < n)
+#pragma unroll 4
+        for (int k = w; k < P; k += 4) v += part[(size_t)k * n + i];
+    sm[w][lane] = v;
+    __syncthreads();
+    if (w == 0 && i < n) out[i] = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
 }
 
 // ---------------------------------------------------------------- C entry
 struct BwdWs { size_t c_h, c_ds, bc, a, d, b, total; };
 static BwdWs bwd_ws(int T, int B, int D, int N, int G) {
-    const int S = sscan_chunks(T, B, D, N, G, 1), np = sscan_np(N), tpg = (D / G + 63) / 64;
+    const int S = sscan_chunks(T, B, D, G), np = sscan_np(N), tpg = (D / G + 63) / 64;
     BwdWs o{};
     size_t at = 0;
     const auto take = [&](size_t floats) { const size_t v = at; at += align256(floats * 4); return v; };
@@ -361,42 +391,35 @@ static void launch_bwd(const SscanArgs& p, hipStream_t stream) {
     hipLaunchKernelGGL((sstate_bwd_kernel<TY, SPL, NB, false>), dim3(p.G * p.tpg, p.B, p.S), dim3(256), 0, stream, p);
 }
 template <typename TY>
-static void launch_bwd_t(const SscanArgs& p, void* dB, void* dC, hipStream_t stream) {
-    if (p.N <= 4) launch_bwd<TY, 1, 1>(p, stream);
+static void launch_bwd_t(const SscanArgs& p, const asr_sscan_desc* d, hipStream_t stream) {
+    if (p.B == 0) {}
+    else if (p.N <= 4) launch_bwd<TY, 1, 1>(p, stream);
     else if (p.N <= 8) launch_bwd<TY, 2, 1>(p, stream);
     else if (p.N <= 16) launch_bwd<TY, 4, 1>(p, stream);
     else if (p.N <= 32) launch_bwd<TY, 4, 2>(p, stream);
     else launch_bwd<TY, 4, 4>(p, stream);
-    const size_t per = (size_t)p.B * p.T * 2 * p.np;
-    if (per)
-        hipLaunchKernelGGL((sscan_dbc_kernel<TY>), dim3((unsigned)((per + 255) / 256), p.G), dim3(256), 0, stream, p.part_bc,
-                           p.T, p.B, p.N, p.np, p.G, p.tpg, p.reverse, p.lens, (TY*)dB, (TY*)dC);
+    const unsigned nbc = (unsigned)(((size_t)p.B * p.T * 2 * p.np + 255) / 256), nd = (p.D + 63) / 64;
+    const unsigned na = (unsigned)(((size_t)p.D * p.N + 63) / 64);
+    hipLaunchKernelGGL((sscan_finish_kernel<TY>), dim3(nbc * p.G + na + (d->dD ? nd : 0) + (d->ddt_bias ? nd : 0)),
+                       dim3(256), 0, stream, p, (TY*)d->dB, (TY*)d->dC, d->dA, d->dD, d->ddt_bias,
+                       nbc, na, nd);
 }
 
 extern "C" int asr_sscan_bwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes, hipStream_t stream) {
     SscanArgs p{};
-    if (int e = sscan_fill(d, &p, 1)) return e;
+    if (int e = sscan_fill(d, &p)) return e;
     if (!d->dA || (d->z && !d->dz && d->T > 0 && d->B > 0)) return ASR_ERR_ARG;
     if (d->T > 0 && d->B > 0 && (!d->dout || !d->ckpt || !d->dx || !d->ddt || !d->dB || !d->dC)) return ASR_ERR_ARG;
-    if (d->G > 65535) return ASR_ERR_LIMIT;
     if (d->dh0 && d->dh0 == d->dh_last) return ASR_ERR_ARG;
+    if ((double)d->B * d->T * 2 * p.np * d->G > 256.0 * 0x7fff0000) return ASR_ERR_LIMIT;        // blocks of a launch
     const BwdWs o = bwd_ws(d->T, d->B, d->D, d->N, d->G);
-    if (d->B && (!ws || ws_bytes < o.total)) return ASR_ERR_WS;
+    if (o.total && (!ws || ws_bytes < o.total)) return ASR_ERR_WS;
     char* base = (char*)ws;
     p.c_h = (float*)(base + o.c_h); p.c_ds = (float*)(base + o.c_ds); p.part_bc = (float*)(base + o.bc);
     p.part_a = (float*)(base + o.a); p.part_d = (float*)(base + o.d); p.part_b = (float*)(base + o.b);
-    int P = 0;
-    if (d->B) {
-        if (d->dtype == ASR_F32) launch_bwd_t<float>(p, d->dB, d->dC, stream);
-        else if (d->dtype == ASR_BF16) launch_bwd_t<bf16_t>(p, d->dB, d->dC, stream);
-        else launch_bwd_t<f16_t>(p, d->dB, d->dC, stream);
-        ASR_CHECK_LAUNCH();
-        P = p.S * p.B;
-    }
-    const size_t n = (size_t)p.D * p.N;
-    sum_partials(p.part_a, n, P, n, d->dA, stream);
-    if (d->dD) sum_partials(p.part_d, p.D, P, p.D, d->dD, stream);
-    if (d->ddt_bias) sum_partials(p.part_b, p.D, P, p.D, d->ddt_bias, stream);
+    if (d->dtype == ASR_F32) launch_bwd_t<float>(p, d, stream);
+    else if (d->dtype == ASR_BF16) launch_bwd_t<bf16_t>(p, d, stream);
+    else launch_bwd_t<f16_t>(p, d, stream);
     ASR_CHECK_LAUNCH();
     return ASR_OK;
 }

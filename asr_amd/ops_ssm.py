@@ -27,134 +27,132 @@ def _fail(msg):
     raise ValueError(msg)
 
 
+_stream = torch._C._cuda_getCurrentRawStream          # the handle alone: torch.cuda.current_stream() makes an object of it
+
+
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _act(name, t, shape, dtype):
-    """an activation: the shape, the call's type, unit stride of the last axis"""
-    if t.shape != shape:
-        _fail('%s: shape %s, expected %s' % (name, tuple(t.shape), tuple(shape)))
-    if t.dtype != dtype:
-        _fail('%s: %s, expected %s like the other activations' % (name, t.dtype, dtype))
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        _fail('%s: the last axis must have stride 1' % name)
+def _act(name, t, shape, dtype, dev):
+    """an activation: the shape, the call's type, the call's device, unit stride of the last axis; -> its strides"""
+    st = t.stride()
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or (st[-1] != 1 and shape[-1] > 1):
+        if t.shape != shape:
+            _fail('%s: shape %s, expected %s' % (name, tuple(t.shape), tuple(shape)))
+        if t.dtype is not dtype:
+            _fail('%s: %s, expected %s like the other activations' % (name, t.dtype, dtype))
+        if t.get_device() == dev:
+            _fail('%s: the last axis must have stride 1' % name)
+        _fail('%s: on %s, unlike the other tensors' % (name, t.device))
+    return st
 
 
-def _par(name, t, shape):
-    """a parameter or a state: float32, contiguous"""
-    if t.shape != shape:
-        _fail('%s: shape %s, expected %s' % (name, tuple(t.shape), tuple(shape)))
-    if t.dtype != torch.float32:
-        _fail('%s: %s, expected torch.float32' % (name, t.dtype))
-    if not t.is_contiguous():
-        _fail('%s: must be contiguous' % name)
+def _par(name, t, shape, dev, like=None):
+    """a parameter or a state: float32 (or the activations' type), contiguous, on the call's device; -> its address"""
+    dtype = like or torch.float32
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != dev:
+        if t.shape != shape:
+            _fail('%s: shape %s, expected %s' % (name, tuple(t.shape), tuple(shape)))
+        if t.dtype is not dtype:
+            _fail('%s: %s, expected %s%s' % (name, t.dtype, dtype, ' like x' if like else ''))
+        if t.get_device() == dev:
+            _fail('%s: must be contiguous, has strides %s' % (name, t.stride()))
+        _fail('%s: on %s, unlike the other tensors' % (name, t.device))
+    return t.data_ptr()
 
 
 def _type(name, t):
-    if t.dtype not in _DTYPES:
+    k = _DTYPES.get(t.dtype)
+    if k is None:
         _fail('%s: %s, expected float32, bfloat16 or float16' % (name, t.dtype))
-    return _DTYPES[t.dtype]
+    return k
 
 
-def _lens(lens, B):
-    if lens is not None and (lens.shape != (B,) or lens.dtype != torch.int32 or not lens.is_contiguous()):
-        _fail('lens: expected %d contiguous int32 values' % B)
-
-
-def _device(first, *others):
-    """all tensors on one GPU; its index"""
-    dev = first.device
-    if dev.type != 'cuda':
+def _gpu(dev):
+    """behind all other checks, which need no GPU"""
+    if dev < 0:
         _fail('tensors must be on the GPU (there is no CPU path)')
-    for t in others:
-        if t is not None and t.device != dev:
-            _fail('tensors on different devices: %s and %s' % (dev, t.device))
-    return dev.index
 
 
-class _On(object):
-    """Makes the tensors' device current for the launches of a call, if it is not."""
-    __slots__ = ('index', 'before')
-
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *a):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _call(what, dev, fn, *args):
+    """fn(*args, the current stream of device dev), with that device current"""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        check(rc, what)
 
 
 # ---------------------------------------------------------------------------------------------- convolution
 def _act_kind(act):
-    if act not in ('silu', None):
+    if act != 'silu' and act is not None:
         _fail("act: 'silu' or None, got %r" % (act,))
     return 1 if act else 0
 
 
-def _conv_args(x, w, bias, state, lens):
+def _taps(w):
+    if w.dim() != 2 or not 2 <= w.shape[1] <= MAX_TAPS:
+        _fail('w: expected (D, K) with 2 <= K <= %d, got %s' % (MAX_TAPS, tuple(w.shape)))
+    return w.shape[1]
+
+
+def _lens(lens, B, dev):
+    if lens is None:
+        return None
+    if lens.shape != (B,) or lens.dtype is not torch.int32 or not lens.is_contiguous():
+        _fail('lens: expected %d contiguous int32 values' % B)
+    if lens.get_device() != dev:
+        _fail('lens: on %s, unlike the other tensors' % lens.device)
+    return lens.data_ptr()
+
+
+def _conv_args(x, w, bias, state, lens, act):
     if x.dim() != 3:
         _fail('x: expected (T, B, D), got %d axes' % x.dim())
     T, B, D = x.shape
-    if w.dim() != 2 or not 2 <= w.shape[1] <= MAX_TAPS:
-        _fail('w: expected (D, K) with 2 <= K <= %d, got %s' % (MAX_TAPS, tuple(w.shape)))
-    K = w.shape[1]
-    dt = _type('x', x)
+    K = _taps(w)
+    kind = _type('x', x)
     if D < 1:
         _fail('x: no channels')
-    _act('x', x, (T, B, D), x.dtype)
-    _par('w', w, (D, K))
-    if bias is not None:
-        _par('bias', bias, (D,))
-    if state is not None:
-        _act('state', state, (K - 1, B, D), x.dtype)
-        if not state.is_contiguous():
-            _fail('state: must be contiguous')
-    _lens(lens, B)
-    return dt, T, B, D, K
+    dev = x.get_device()
+    st = _act('x', x, (T, B, D), x.dtype, dev)
+    pw = _par('w', w, (D, K), dev)
+    pb = _par('bias', bias, (D,), dev) if bias is not None else None
+    ps = _par('state', state, (K - 1, B, D), dev, x.dtype) if state is not None else None
+    return kind, T, B, D, K, dev, st, pw, pb, ps, _lens(lens, B, dev), _act_kind(act)
 
 
 def causal_conv_fwd(x, w, bias=None, state=None, lens=None, act='silu', reverse=False, want_state=False):
     """out[s] = act(bias + sum_k w[:, k] x[s - (K-1) + k]) over the valid frames s of every row; x (T, B, D), w (D, K).
     state (K-1, B, D): the frames in front of the first one (None: zeros).  -> (out, the state behind the last valid frame
     if want_state, else None)."""
-    dt, T, B, D, K = _conv_args(x, w, bias, state, lens)
-    kind = _act_kind(act)
-    dev = _device(x, w, bias, state, lens)
+    kind, T, B, D, K, dev, st, pw, pb, ps, pl, silu = _conv_args(x, w, bias, state, lens, act)
+    _gpu(dev)
     out = torch.empty((T, B, D), dtype=x.dtype, device=x.device)
     new = torch.empty((K - 1, B, D), dtype=x.dtype, device=x.device) if want_state else None
-    with _On(dev) as st:
-        check(_lib.lib().asr_conv_fwd(dt, T, B, D, K, _p(x), x.stride(0), x.stride(1), _p(w), _p(bias), _p(state), _p(lens),
-                                      kind, int(reverse), _p(out), B * D, D, _p(new), st), 'asr_conv_fwd')
+    _call('asr_conv_fwd', dev, _lib.lib().asr_conv_fwd, kind, T, B, D, K, x.data_ptr(), st[0], st[1], pw, pb, ps, pl, silu,
+          int(reverse), out.data_ptr(), B * D, D, _p(new))
     return out, new
 
 
 def causal_conv_bwd(dout, x, w, bias=None, state=None, lens=None, act='silu', reverse=False, dstate_out=None):
     """Gradients of causal_conv_fwd for the gradient dout of its output (and dstate_out of the state it returned):
     {'x', 'w', 'bias', 'state'}; 'bias' / 'state' are None when there was none."""
-    dt, T, B, D, K = _conv_args(x, w, bias, state, lens)
-    kind = _act_kind(act)
-    _act('dout', dout, (T, B, D), x.dtype)
-    if dstate_out is not None:
-        _act('dstate_out', dstate_out, (K - 1, B, D), x.dtype)
-        if not dstate_out.is_contiguous():
-            _fail('dstate_out: must be contiguous')
-    dev = _device(x, dout, w, bias, state, lens, dstate_out)
+    kind, T, B, D, K, dev, st, pw, pb, ps, pl, silu = _conv_args(x, w, bias, state, lens, act)
+    so = _act('dout', dout, (T, B, D), x.dtype, dev)
+    pd = _par('dstate_out', dstate_out, (K - 1, B, D), dev, x.dtype) if dstate_out is not None else None
+    _gpu(dev)
+    L = _lib.lib()
     dx = torch.empty((T, B, D), dtype=x.dtype, device=x.device)
     dwb = torch.empty(D * (K + 1), dtype=torch.float32, device=x.device)
     ds = torch.empty((K - 1, B, D), dtype=x.dtype, device=x.device) if state is not None else None
-    L = _lib.lib()
-    with _On(dev) as st:
-        ws = torch.empty(L.asr_conv_bwd_ws_bytes(T, B, D, K), dtype=torch.uint8, device=x.device)
-        check(L.asr_conv_bwd(dt, T, B, D, K, _p(dout), dout.stride(0), dout.stride(1), _p(x), x.stride(0), x.stride(1),
-                             _p(w), _p(bias), _p(state), _p(lens), kind, int(reverse), _p(dstate_out), _p(dx), _p(dwb),
-                             _p(ds), _p(ws), ws.numel(), st), 'asr_conv_bwd')
+    need = L.asr_conv_bwd_ws_bytes(T, B, D, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _call('asr_conv_bwd', dev, L.asr_conv_bwd, kind, T, B, D, K, dout.data_ptr(), so[0], so[1], x.data_ptr(), st[0], st[1], pw,
+          pb, ps, pl, silu, int(reverse), pd, dx.data_ptr(), dwb.data_ptr(), _p(ds), ws.data_ptr(), need)
     return {'x': dx, 'w': dwb[:D * K].view(D, K), 'bias': dwb[D * K:] if bias is not None else None, 'state': ds}
 
 
@@ -163,67 +161,56 @@ def causal_conv_step(x, state, w, bias=None, act='silu'):
     frame."""
     if x.dim() != 2:
         _fail('x: expected (B, D), got %d axes' % x.dim())
-    B, D = x.shape
-    if w.dim() != 2 or not 2 <= w.shape[1] <= MAX_TAPS:
-        _fail('w: expected (D, K) with 2 <= K <= %d, got %s' % (MAX_TAPS, tuple(w.shape)))
-    K = w.shape[1]
-    dt = _type('x', x)
+    sh = x.shape
+    B, D = sh
+    K = _taps(w)
+    ty, dev = x.dtype, x.get_device()
+    kind = _type('x', x)
     if D < 1:
         _fail('x: no channels')
-    _act('x', x, (B, D), x.dtype)
-    _par('w', w, (D, K))
-    if bias is not None:
-        _par('bias', bias, (D,))
-    _act('state', state, (K - 1, B, D), x.dtype)
-    if not state.is_contiguous():
-        _fail('state: must be contiguous')
-    kind = _act_kind(act)
-    dev = _device(x, state, w, bias)
-    out = torch.empty((B, D), dtype=x.dtype, device=x.device)
-    with _On(dev) as st:
-        check(_lib.lib().asr_conv_step(dt, B, D, K, x.data_ptr(), x.stride(0), state.data_ptr(), w.data_ptr(), _p(bias),
-                                       kind, out.data_ptr(), D, st), 'asr_conv_step')
+    st = _act('x', x, sh, ty, dev)
+    pw = _par('w', w, (D, K), dev)
+    pb = _par('bias', bias, (D,), dev) if bias is not None else None
+    ps = _par('state', state, (K - 1, B, D), dev, ty)
+    silu = _act_kind(act)
+    _gpu(dev)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _call('asr_conv_step', dev, _lib.lib().asr_conv_step, kind, B, D, K, x.data_ptr(), st[0], ps, pw, pb, silu, out.data_ptr(), D)
     return out
 
 
 # ---------------------------------------------------------------------------------------------- selective scan
-def _scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens):
-    if x.dim() != 3:
-        _fail('x: expected (T, B, D), got %d axes' % x.dim())
-    T, B, Dn = x.shape
+def _states(A, Bm, Dn, axes):
+    """N, G"""
     if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATES:
         _fail('A: expected (D, N) with 1 <= N <= %d, got %s' % (MAX_STATES, tuple(A.shape)))
-    N = A.shape[1]
-    if Bm.dim() != 4:
-        _fail('Bm: expected (T, B, G, N), got %d axes' % Bm.dim())
-    G = Bm.shape[2]
+    if Bm.dim() != axes:
+        _fail('Bm: expected %s, got %d axes' % ('(T, B, G, N)' if axes == 4 else '(B, G, N)', Bm.dim()))
+    G = Bm.shape[-2]
     if Dn < 1 or G < 1 or Dn % G:
         _fail('Bm: %d groups do not divide %d channels' % (G, Dn))
-    kind = _type('x', x)
-    ty = x.dtype
-    _act('x', x, (T, B, Dn), ty)
-    _act('dt', dt, (T, B, Dn), ty)
-    _par('A', A, (Dn, N))
-    _act('Bm', Bm, (T, B, G, N), ty)
-    _act('Cm', Cm, (T, B, G, N), ty)
-    if z is not None:
-        _act('z', z, (T, B, Dn), ty)
-    if D is not None:
-        _par('D', D, (Dn,))
-    if dt_bias is not None:
-        _par('dt_bias', dt_bias, (Dn,))
-    if h0 is not None:
-        _par('h0', h0, (B, Dn, N))
-    _lens(lens, B)
-    return kind, T, B, Dn, N, G
+    return A.shape[1], G
 
 
-def _scan_desc(kind, T, B, Dn, N, G, x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens, softplus, reverse):
-    return (T, B, Dn, N, G, kind, int(reverse), int(softplus), _p(lens),
-            x.data_ptr(), x.stride(0), x.stride(1), dt.data_ptr(), dt.stride(0), dt.stride(1),
-            _p(z), z.stride(0) if z is not None else 0, z.stride(1) if z is not None else 0,
-            Bm.data_ptr(), Bm.stride(0), Bm.stride(1), Bm.stride(2), Cm.data_ptr(), Cm.stride(0), Cm.stride(1), Cm.stride(2),
-            A.data_ptr(), _p(D), _p(dt_bias), _p(h0))
+def _scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens, softplus, reverse):
+    """the sizes, the device, and the descriptor's members up to h0"""
+    if x.dim() != 3:
+        _fail('x: expected (T, B, D), got %d axes' % x.dim())
+    sh = T, B, Dn = x.shape
+    N, G = _states(A, Bm, Dn, 4)
+    kind, ty, dev = _type('x', x), x.dtype, x.get_device()
+    sx = _act('x', x, sh, ty, dev)
+    sd = _act('dt', dt, sh, ty, dev)
+    pA = _par('A', A, (Dn, N), dev)
+    sB = _act('Bm', Bm, (T, B, G, N), ty, dev)
+    sC = _act('Cm', Cm, (T, B, G, N), ty, dev)
+    pz, sz = (z.data_ptr(), _act('z', z, sh, ty, dev)) if z is not None else (None, (0, 0))
+    pD = _par('D', D, (Dn,), dev) if D is not None else None
+    pb = _par('dt_bias', dt_bias, (Dn,), dev) if dt_bias is not None else None
+    ph = _par('h0', h0, (B, Dn, N), dev) if h0 is not None else None
+    return (T, B, Dn, N, G), dev, (T, B, Dn, N, G, kind, int(reverse), int(softplus), _lens(lens, B, dev), x.data_ptr(), sx[0],
+                                   sx[1], dt.data_ptr(), sd[0], sd[1], pz, sz[0], sz[1], Bm.data_ptr(), sB[0], sB[1], sB[2],
+                                   Cm.data_ptr(), sC[0], sC[1], sC[2], pA, pD, pb, ph)
 
 
 def selective_scan_fwd(x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, h0=None, lens=None, softplus=True, reverse=False,
@@ -234,19 +221,17 @@ def selective_scan_fwd(x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, h0=None, 
     x, dt, z (T, B, D); A (D, N), N <= 64; Bm, Cm (T, B, G, N), shared by the D / G channels of a group; D, dt_bias (D,);
     h0 (B, D, N) (None: zeros).  -> (out (T, B, D), the state behind the last valid frame (B, D, N), what
     selective_scan_bwd needs if train, else None)."""
-    a = _scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens)
-    kind, T, B, Dn, N, G = a
-    dev = _device(x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens)
+    (T, B, Dn, N, G), dev, members = _scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens, softplus, reverse)
+    _gpu(dev)
     L = _lib.lib()
-    out = torch.empty((T, B, Dn), dtype=x.dtype, device=x.device)
-    h = torch.empty((B, Dn, N), dtype=torch.float32, device=x.device)
-    saved = torch.empty(L.asr_sscan_ckpt_floats(T, B, Dn, N), dtype=torch.float32, device=x.device) if train else None
-    desc = _lib.SscanDesc(*_scan_desc(*a, x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens, softplus, reverse),
-                          out.data_ptr(), B * Dn, Dn, h.data_ptr(), _p(saved))
-    with _On(dev) as st:
-        need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        check(L.asr_sscan_fwd(C.byref(desc), _p(ws), need, st), 'asr_sscan_fwd')
+    f32, on = torch.float32, x.device
+    out = torch.empty((T, B, Dn), dtype=x.dtype, device=on)
+    h = torch.empty((B, Dn, N), dtype=f32, device=on)
+    saved = torch.empty(L.asr_sscan_ckpt_floats(T, B, Dn, N), dtype=f32, device=on) if train else None
+    need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=on) if need else None
+    desc = _lib.SscanDesc(*members, out.data_ptr(), B * Dn, Dn, h.data_ptr(), _p(saved))
+    _call('asr_sscan_fwd', dev, L.asr_sscan_fwd, C.byref(desc), _p(ws), need)
     return out, h, saved
 
 
@@ -255,33 +240,28 @@ def selective_scan_bwd(dout, x, dt, A, Bm, Cm, saved, D=None, z=None, dt_bias=No
     """Gradients of selective_scan_fwd(..., train=True) called with the same arguments, for the gradient dout of its output
     (and dh_last of the state it returned): {'x', 'dt', 'A', 'B', 'C', 'D', 'z', 'dt_bias', 'h0'}, None where the argument
     was.  `saved` is what the forward call returned."""
-    a = _scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens)
-    kind, T, B, Dn, N, G = a
-    _act('dout', dout, (T, B, Dn), x.dtype)
+    (T, B, Dn, N, G), dev, members = _scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens, softplus, reverse)
+    so = _act('dout', dout, (T, B, Dn), x.dtype, dev)
     L = _lib.lib()
-    if saved is None or saved.dtype != torch.float32 or saved.numel() != L.asr_sscan_ckpt_floats(T, B, Dn, N) or \
-            not saved.is_contiguous():
+    if saved is None or saved.shape != (L.asr_sscan_ckpt_floats(T, B, Dn, N),):
         _fail('saved: not what selective_scan_fwd(..., train=True) returned for these shapes')
-    if dh_last is not None:
-        _par('dh_last', dh_last, (B, Dn, N))
-    dev = _device(x, dout, dt, A, Bm, Cm, saved, D, z, dt_bias, h0, lens, dh_last)
-
-    def new(shape, dtype):
-        return torch.empty(shape, dtype=dtype, device=x.device)
-    ty, f32 = x.dtype, torch.float32
-    g = {'x': new((T, B, Dn), ty), 'dt': new((T, B, Dn), ty), 'A': new((Dn, N), f32), 'B': new((T, B, G, N), ty),
-         'C': new((T, B, G, N), ty), 'D': new((Dn,), f32) if D is not None else None,
-         'z': new((T, B, Dn), ty) if z is not None else None,
-         'dt_bias': new((Dn,), f32) if dt_bias is not None else None,
-         'h0': new((B, Dn, N), f32) if h0 is not None else None}
-    desc = _lib.SscanDesc(*_scan_desc(*a, x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens, softplus, reverse),
-                          None, 0, 0, None, saved.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), _p(dh_last),
-                          _p(g['x']), _p(g['dt']), _p(g['z']), _p(g['B']), _p(g['C']), _p(g['A']), _p(g['D']),
-                          _p(g['dt_bias']), _p(g['h0']))
-    with _On(dev) as st:
-        need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 1)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        check(L.asr_sscan_bwd(C.byref(desc), _p(ws), need, st), 'asr_sscan_bwd')
+    ps = _par('saved', saved, saved.shape, dev)
+    ph = _par('dh_last', dh_last, (B, Dn, N), dev) if dh_last is not None else None
+    _gpu(dev)
+    ty, f32, on = x.dtype, torch.float32, x.device
+    wide, states = (T, B, Dn), (T, B, G, N)
+    g = {'x': torch.empty(wide, dtype=ty, device=on), 'dt': torch.empty(wide, dtype=ty, device=on),
+         'A': torch.empty((Dn, N), dtype=f32, device=on), 'B': torch.empty(states, dtype=ty, device=on),
+         'C': torch.empty(states, dtype=ty, device=on), 'D': torch.empty_like(D) if D is not None else None,
+         'z': torch.empty(wide, dtype=ty, device=on) if z is not None else None,
+         'dt_bias': torch.empty_like(dt_bias) if dt_bias is not None else None,
+         'h0': torch.empty_like(h0) if h0 is not None else None}
+    need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=on)
+    desc = _lib.SscanDesc(*members, None, 0, 0, None, ps, dout.data_ptr(), so[0], so[1], ph, g['x'].data_ptr(),
+                          g['dt'].data_ptr(), _p(g['z']), g['B'].data_ptr(), g['C'].data_ptr(), g['A'].data_ptr(),
+                          _p(g['D']), _p(g['dt_bias']), _p(g['h0']))
+    _call('asr_sscan_bwd', dev, L.asr_sscan_bwd, C.byref(desc), ws.data_ptr(), need)
     return g
 
 
@@ -289,94 +269,72 @@ def selective_scan_step(h, x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, softp
     """One frame of selective_scan_fwd: h (B, D, N) moves on in place; x, dt, z (B, D); Bm, Cm (B, G, N).  -> out (B, D)."""
     if x.dim() != 2:
         _fail('x: expected (B, D), got %d axes' % x.dim())
-    B, Dn = x.shape
-    if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATES:
-        _fail('A: expected (D, N) with 1 <= N <= %d, got %s' % (MAX_STATES, tuple(A.shape)))
-    N = A.shape[1]
-    if Bm.dim() != 3:
-        _fail('Bm: expected (B, G, N), got %d axes' % Bm.dim())
-    G = Bm.shape[1]
-    if Dn < 1 or G < 1 or Dn % G:
-        _fail('Bm: %d groups do not divide %d channels' % (G, Dn))
-    kind = _type('x', x)
-    ty = x.dtype
-    _act('x', x, (B, Dn), ty)
-    _act('dt', dt, (B, Dn), ty)
-    _par('A', A, (Dn, N))
-    _act('Bm', Bm, (B, G, N), ty)
-    _act('Cm', Cm, (B, G, N), ty)
-    if z is not None:
-        _act('z', z, (B, Dn), ty)
-    if D is not None:
-        _par('D', D, (Dn,))
-    if dt_bias is not None:
-        _par('dt_bias', dt_bias, (Dn,))
-    _par('h', h, (B, Dn, N))
-    dev = _device(x, h, dt, A, Bm, Cm, D, z, dt_bias)
-    out = torch.empty((B, Dn), dtype=ty, device=x.device)
-    with _On(dev) as st:
-        check(_lib.lib().asr_sscan_step(kind, B, Dn, N, G, h.data_ptr(), x.data_ptr(), x.stride(0), dt.data_ptr(),
-                                        dt.stride(0), A.data_ptr(), Bm.data_ptr(), Bm.stride(0), Bm.stride(1),
-                                        Cm.data_ptr(), Cm.stride(0), Cm.stride(1), _p(D), _p(z),
-                                        z.stride(0) if z is not None else 0, _p(dt_bias), int(softplus), out.data_ptr(),
-                                        Dn, st), 'asr_sscan_step')
+    sh = B, Dn = x.shape
+    N, G = _states(A, Bm, Dn, 3)
+    kind, ty, dev = _type('x', x), x.dtype, x.get_device()
+    sx = _act('x', x, sh, ty, dev)
+    sd = _act('dt', dt, sh, ty, dev)
+    pA = _par('A', A, (Dn, N), dev)
+    sB = _act('Bm', Bm, (B, G, N), ty, dev)
+    sC = _act('Cm', Cm, (B, G, N), ty, dev)
+    pz, sz = (z.data_ptr(), _act('z', z, sh, ty, dev)[0]) if z is not None else (None, 0)
+    pD = _par('D', D, (Dn,), dev) if D is not None else None
+    pb = _par('dt_bias', dt_bias, (Dn,), dev) if dt_bias is not None else None
+    ph = _par('h', h, (B, Dn, N), dev)
+    _gpu(dev)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _call('asr_sscan_step', dev, _lib.lib().asr_sscan_step, kind, B, Dn, N, G, ph, x.data_ptr(), sx[0], dt.data_ptr(), sd[0], pA,
+          Bm.data_ptr(), sB[0], sB[1], Cm.data_ptr(), sC[0], sC[1], pD, pz, sz, pb, 1 if softplus else 0, out.data_ptr(), Dn)
     return out
 
 
 # ---------------------------------------------------------------------------------------------- norm
+def _rows(x):
+    if x.dim() != 2:
+        _fail('x: expected (rows, n), got %d axes' % x.dim())
+    if x.shape[1] < 1:
+        _fail('x: no columns')
+    return x.shape, _type('x', x), x.dtype, x.get_device()
+
+
 def add_rms_norm_fwd(x, w, residual=None, eps=1e-6):
     """r = x + residual,  y = r / sqrt(mean(r^2) + eps) * w over rows; x, residual (rows, n) with unit column stride, w (n,).
     -> (y, r in the type of x (x itself without a residual), 1 / sqrt(...) of every row for the backward pass)."""
-    if x.dim() != 2:
-        _fail('x: expected (rows, n), got %d axes' % x.dim())
-    rows, n = x.shape
-    if n < 1:
-        _fail('x: no columns')
-    kind = _type('x', x)
-    _act('x', x, (rows, n), x.dtype)
-    _par('w', w, (n,))
-    if residual is not None:
-        _act('residual', residual, (rows, n), x.dtype)
+    sh, kind, ty, dev = _rows(x)
+    rows, n = sh
+    sx = _act('x', x, sh, ty, dev)
+    pw = _par('w', w, (n,), dev)
+    pr, sr = (residual.data_ptr(), _act('residual', residual, sh, ty, dev)[0]) if residual is not None else (None, 0)
     if not eps >= 0:
         _fail('eps: %r is negative' % (eps,))
-    dev = _device(x, w, residual)
-    y = torch.empty((rows, n), dtype=x.dtype, device=x.device)
-    r = torch.empty((rows, n), dtype=x.dtype, device=x.device) if residual is not None else None
+    _gpu(dev)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    r = torch.empty_like(y) if pr is not None else None
     rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    with _On(dev) as st:
-        check(_lib.lib().asr_rms_norm_fwd(kind, x.data_ptr(), x.stride(0), _p(residual),
-                                          residual.stride(0) if residual is not None else 0, w.data_ptr(), rows, n, eps,
-                                          y.data_ptr(), _p(r), rstd.data_ptr(), st), 'asr_rms_norm_fwd')
+    _call('asr_rms_norm_fwd', dev, _lib.lib().asr_rms_norm_fwd, kind, x.data_ptr(), sx[0], pr, sr, pw, rows, n, eps,
+          y.data_ptr(), _p(r), rstd.data_ptr())
     return y, (x if r is None else r), rstd
 
 
 def add_rms_norm_bwd(dy, x, w, rstd, residual=None, dres=None):
     """Gradients of add_rms_norm_fwd(x, w, residual): dy (rows, n) of y, dres (rows, n) of r (None: r went nowhere else),
     rstd as the forward call returned it.  -> (dr, dw); dr is the gradient of x and of the residual alike."""
-    if x.dim() != 2:
-        _fail('x: expected (rows, n), got %d axes' % x.dim())
-    rows, n = x.shape
-    if n < 1:
-        _fail('x: no columns')
-    kind = _type('x', x)
-    _act('x', x, (rows, n), x.dtype)
-    _act('dy', dy, (rows, n), x.dtype)
-    _par('w', w, (n,))
-    _par('rstd', rstd, (rows,))
-    if residual is not None:
-        _act('residual', residual, (rows, n), x.dtype)
-    if dres is not None:
-        _act('dres', dres, (rows, n), x.dtype)
-    dev = _device(x, dy, w, rstd, residual, dres)
-    dx = torch.empty((rows, n), dtype=x.dtype, device=x.device)
-    dw = torch.empty((n,), dtype=torch.float32, device=x.device)
+    sh, kind, ty, dev = _rows(x)
+    rows, n = sh
+    sx = _act('x', x, sh, ty, dev)
+    sy = _act('dy', dy, sh, ty, dev)
+    pw = _par('w', w, (n,), dev)
+    ps = _par('rstd', rstd, (rows,), dev)
+    pr, sr = (residual.data_ptr(), _act('residual', residual, sh, ty, dev)[0]) if residual is not None else (None, 0)
+    pd, sd = (dres.data_ptr(), _act('dres', dres, sh, ty, dev)[0]) if dres is not None else (None, 0)
+    _gpu(dev)
     L = _lib.lib()
-    with _On(dev) as st:
-        ws = torch.empty(L.asr_rms_norm_bwd_ws_bytes(rows, n), dtype=torch.uint8, device=x.device)
-        check(L.asr_rms_norm_bwd(kind, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _p(residual),
-                                 residual.stride(0) if residual is not None else 0, w.data_ptr(), rstd.data_ptr(),
-                                 _p(dres), dres.stride(0) if dres is not None else 0, rows, n, dx.data_ptr(), dw.data_ptr(),
-                                 _p(ws), ws.numel(), st), 'asr_rms_norm_bwd')
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dw = torch.empty_like(w)
+    need = L.asr_rms_norm_bwd_ws_bytes(rows, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _call('asr_rms_norm_bwd', dev, L.asr_rms_norm_bwd, kind, dy.data_ptr(), sy[0], x.data_ptr(), sx[0], pr, sr, pw, ps, pd, sd,
+          rows, n, dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), need)
     return dx, dw
 
 
@@ -384,23 +342,36 @@ def add_rms_norm_bwd(dy, x, w, rstd, residual=None, dres=None):
 def clip_list(tensors, max_norm, eps=1e-7):
     """-> ([t * clip(norm, 0, max_norm) / (eps + norm) for t in tensors], norm (1,)), norm the root of the sum of all squares:
     libs/lasagne_libs/updates.py:845-855 for gradients that do not lie in one buffer.  float32, bfloat16 and float16 tensors of
-    any shape may be mixed; the multiplier stays on the device."""
+    any shape may be mixed; the multiplier stays on the device.  The results of one type share one buffer."""
     tensors = list(tensors)
     if not tensors:
         _fail('tensors: none given')
     if not max_norm >= 0 or not eps >= 0:
         _fail('max_norm %r and eps %r must not be negative' % (max_norm, eps))
     kinds = [_type('tensors[%d]' % i, t) for i, t in enumerate(tensors)]
-    dev = _device(*tensors)
-    n = len(tensors)
+    dev = tensors[0].get_device()
+    for i, t in enumerate(tensors):
+        if t.get_device() != dev:
+            _fail('tensors[%d]: on %s, unlike the others' % (i, t.device))
+    _gpu(dev)
+    n, on = len(tensors), tensors[0].device
     src = [t if t.is_contiguous() else t.contiguous() for t in tensors]
-    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in src]
-    norm = torch.empty((1,), dtype=torch.float32, device=tensors[0].device)
-    sizes = (C.c_longlong * n)(*[t.numel() for t in src])
+    sizes = [t.numel() for t in src]
+    out, dst = [None] * n, [0] * n
+    for dtype, kind in _DTYPES.items():
+        mine = [i for i in range(n) if kinds[i] == kind]
+        if not mine:
+            continue
+        flat = torch.empty(sum([sizes[i] for i in mine]), dtype=dtype, device=on)
+        at, e = flat.data_ptr(), flat.element_size()
+        for i, view in zip(mine, torch._C._nn.unflatten_dense_tensors(flat, [src[i] for i in mine])):
+            out[i], dst[i] = view, at
+            at += sizes[i] * e
     L = _lib.lib()
-    with _On(dev) as st:
-        ws = torch.empty(L.asr_clip_list_ws_bytes(n, sizes), dtype=torch.uint8, device=norm.device)
-        check(L.asr_clip_list(n, (C.c_int * n)(*kinds), (C.c_void_p * n)(*[t.data_ptr() for t in src]),
-                              (C.c_void_p * n)(*[t.data_ptr() for t in out]), sizes, max_norm, eps, norm.data_ptr(),
-                              ws.data_ptr(), ws.numel(), st), 'asr_clip_list')
+    csizes = (C.c_longlong * n)(*sizes)
+    need = L.asr_clip_list_ws_bytes(n, csizes)
+    norm = torch.empty((1,), dtype=torch.float32, device=on)
+    ws = torch.empty(need, dtype=torch.uint8, device=on)
+    _call('asr_clip_list', dev, L.asr_clip_list, n, (C.c_int * n)(*kinds), (C.c_void_p * n)(*[t.data_ptr() for t in src]),
+          (C.c_void_p * n)(*dst), csizes, max_norm, eps, norm.data_ptr(), ws.data_ptr(), need)
     return out, norm
