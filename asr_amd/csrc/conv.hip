@@ -1,8 +1,9 @@
 // Short causal depthwise convolution over time with an optional SiLU, forward, backward and for single frames.
 //   pre[s,d] = bias[d] + sum_k w[d,k] x[s-(K-1)+k, d],   out = silu(pre) or pre
 // s counts the valid frames of a row in walking order; s < 0 is the carried state.  HBM-bound: one pass over x (and dout).
-// A thread owns V channels (16 bytes) and a run of frames and keeps the K-frame window in registers, so a frame is loaded
-// once per run plus the K-1 frames in front of it.
+// A thread owns V channels and a run of frames and keeps the K-frame window in registers, so a frame is loaded once per run plus
+// the K-1 frames in front of it.  Measured at T 4096, B 16, D 2048, bf16, K 4: forward 129 us (4.2 TB/s of the 0.54 GB it has to
+// move), backward 200 us (4.0 TB/s of 0.81 GB); one f32 frame of 16 x 1024 channels 3.3 us, the launch.
 #include "seq_common.h"
 
 struct ConvArgs {
@@ -19,6 +20,9 @@ struct ConvArgs {
     float* part;                // (runs groups * B, K+1, D)
 };
 
+// frames a thread walks: a multiple of K near n
+__host__ __device__ constexpr int conv_run(int K, int n) { return (n + K - 1) / K * K; }
+
 // the input at walking position s (>= -(K-1)) of row b
 template <typename T, int V, int K>
 __device__ __forceinline__ void load_x(const ConvArgs& p, int s, int len, int b, int d, float* o) {
@@ -33,14 +37,22 @@ __device__ __forceinline__ void load_x(const ConvArgs& p, int s, int len, int b,
     }
 }
 
+template <typename T, int V> using Raw = typename Vec<T, V>::type;
+template <typename T, int V> __device__ __forceinline__ float raw_at(const Raw<T, V>& r, int e) {
+    if constexpr (V == 1) return (float)r; else return (float)r[e];
+}
+
+// Frames are taken K at a time, so that a frame's place in the window (s mod K) is known when the code is compiled and nothing
+// is moved from register to register.
 template <typename T, int V, int K>
-__global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p, int run) {
+__global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p) {
     const int d = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
     const int b = blockIdx.z;
-    const int s0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * run;
+    constexpr int RUN = conv_run(K, 16);
+    const int s0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * RUN;
     if (d >= p.D) return;
     const int len = row_len(p.lens, b, p.T);
-    const int s1 = min(s0 + run, p.T);
+    const int s1 = min(s0 + RUN, p.T);
     T* out = (T*)p.out + b * p.o_sb + d;
     if (s0 < len) {
         float w[K][V], win[K][V], bias[V];
@@ -50,24 +62,38 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p, int run) {
 #pragma unroll
             for (int k = 0; k < K; ++k) w[k][e] = p.w[(size_t)(d + e) * K + k];
         }
+        // the frame at s0 + i sits in win[(i + K - 1) % K]
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) load_x<T, V, K>(p, s0 - (K - 1) + k, len, b, d, win[k]);
         const int se = min(s1, len);
-        for (int s = s0; s < se; ++s) {
-            load_x<T, V, K>(p, s, len, b, d, win[K - 1]);
+        const auto frame = [&](int s, int j) {
             float y[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 float a = bias[e];
 #pragma unroll
-                for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][e], win[k][e], a);
+                for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][e], win[(j + k) % K][e], a);
                 y[e] = p.act ? silu_(a) : a;
             }
             stv<T, V>(out + (p.reverse ? len - 1 - s : s) * p.o_st, y);
+        };
+        int s = s0;
+        for (; s + K <= se; s += K) {
+            float nx[K][V];
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k)
+            for (int j = 0; j < K; ++j) load_x<T, V, K>(p, s + j, len, b, d, nx[j]);
 #pragma unroll
-                for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e];
+            for (int j = 0; j < K; ++j) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) win[(j + K - 1) % K][e] = nx[j][e];
+                frame(s + j, j);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) {
+            if (s + j >= se) break;
+            load_x<T, V, K>(p, s + j, len, b, d, win[(j + K - 1) % K]);
+            frame(s + j, j);
         }
     }
     const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -83,18 +109,19 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p, int run) {
     }
 }
 
-// dx and the parts of dw / db.  A thread walks e = s0 .. s0+run+K-2: it forms dpre[e], adds dpre[e] x to dw for the frames it
-// owns (e < s0+run) and, K-1 frames later, has all the terms of dx[e-(K-1)].
+// dx and the parts of dw / db.  A thread walks q = s0 .. s0+run+K-2: it forms dpre[q], adds dpre[q] x to dw for the frames it
+// owns (q < s0+run) and, K-1 frames later, has all the terms of dx[q-(K-1)].
 template <typename T, int V, int K>
-__global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p, int run) {
+__global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p) {
     __shared__ float sm[3][K + 1][64 * V];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int d = (blockIdx.x * 64 + lane) * V;
     const int b = blockIdx.z;
-    const int s0 = (blockIdx.y * 4 + wv) * run;
+    constexpr int RUN = conv_run(K, 32);
+    const int s0 = (blockIdx.y * 4 + wv) * RUN;
     const bool on = d < p.D;
     const int len = row_len(p.lens, b, p.T);
-    const int s1 = min(s0 + run, p.T);
+    const int s1 = min(s0 + RUN, p.T);
     float dw[K + 1][V];
 #pragma unroll
     for (int k = 0; k <= K; ++k)
@@ -108,47 +135,35 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p, int run) {
 #pragma unroll
             for (int k = 0; k < K; ++k) { w[k][e] = p.w[(size_t)(d + e) * K + k]; dp[k][e] = 0.f; }
         }
+        // x and dpre of the frame at s0 + i sit in [(i + K - 1) % K]
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) load_x<T, V, K>(p, s0 - (K - 1) + k, len, b, d, win[k]);
         const int own = min(s1, len);              // dx rows of this thread: [s0, own), and the state rows if s0 == 0
-        for (int q = s0; q < own + K - 1; ++q) {
+        const T* pdo = (const T*)p.dout + b * p.do_sb + d;
+        // dpre of frame q (its x is in the window) from dout, and its share of dw
+        const auto gradient = [&](int j, const float (&g)[V], bool mine) {
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k)
+            for (int e = 0; e < V; ++e) {
+                float a = bias[e], v = g[e];
 #pragma unroll
-                for (int e = 0; e < V; ++e) dp[k][e] = dp[k + 1][e];
-            if (q < len) {
-                float g[V];
-                load_x<T, V, K>(p, q, len, b, d, win[K - 1]);
-                ldv<T, V>((const T*)p.dout + (p.reverse ? len - 1 - q : q) * p.do_st + b * p.do_sb + d, g);
+                for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][e], win[(j + k) % K][e], a);
+                if (p.act) v *= dsilu_(a, sigm_(a));
+                dp[(j + K - 1) % K][e] = v;
+                if (mine) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    float a = bias[e];
-#pragma unroll
-                    for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][e], win[k][e], a);
-                    if (p.act) g[e] *= dsilu_(a, sigm_(a));
-                    dp[K - 1][e] = g[e];
-                    if (q < own) {
-#pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][e] = __builtin_fmaf(g[e], win[k][e], dw[k][e]);
-                        dw[K][e] += g[e];
-                    }
+                    for (int k = 0; k < K; ++k) dw[k][e] = __builtin_fmaf(v, win[(j + k) % K][e], dw[k][e]);
+                    dw[K][e] += v;
                 }
-#pragma unroll
-                for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) dp[K - 1][e] = 0.f;
             }
-            const int s = q - (K - 1);             // dx[s] = sum_j w[K-1-j] dpre[s+j]
-            if (s < s0 && s0 != 0) continue;
+        };
+        // dx[s], s = q - (K-1): sum_i w[K-1-i] dpre[s+i]
+        const auto emit = [&](int s, int j) {
             float o[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 o[e] = 0.f;
 #pragma unroll
-                for (int j = 0; j < K; ++j) o[e] = __builtin_fmaf(w[K - 1 - j][e], dp[j][e], o[e]);
+                for (int i = 0; i < K; ++i) o[e] = __builtin_fmaf(w[K - 1 - i][e], dp[(j + i) % K][e], o[e]);
             }
             const int r = s - (len - (K - 1));     // this position's row of the carried-out state
             if (p.dstate_out && r >= 0) {
@@ -159,6 +174,50 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p, int run) {
             }
             if (s >= 0) stv<T, V>((T*)p.dx + ((size_t)(p.reverse ? len - 1 - s : s) * p.B + b) * p.D + d, o);
             else if (p.dstate) stv<T, V>((T*)p.dstate + ((size_t)(s + K - 1) * p.B + b) * p.D + d, o);
+        };
+        // whole windows: the next one is on its way while one is worked on
+        int q = s0;
+        Raw<T, V> nx[K], ng[K];
+        const T* pxb = (const T*)p.x + b * p.x_sb + d;
+        const auto fetch = [&](int q) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                const long long f = p.reverse ? len - 1 - q - j : q + j;
+                nx[j] = *(const Raw<T, V>*)(pxb + f * p.x_st);
+                ng[j] = *(const Raw<T, V>*)(pdo + f * p.do_st);
+            }
+        };
+        if (q + K <= own) fetch(q);
+        for (; q + K <= own; q += K) {
+            Raw<T, V> cx[K], cg[K];
+#pragma unroll
+            for (int j = 0; j < K; ++j) { cx[j] = nx[j]; cg[j] = ng[j]; }
+            if (q + 2 * K <= own) fetch(q + K);
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                float g[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) { win[(j + K - 1) % K][e] = raw_at<T, V>(cx[j], e); g[e] = raw_at<T, V>(cg[j], e); }
+                gradient(j, g, true);
+                if (q + j - (K - 1) >= s0 || s0 == 0) emit(q + j - (K - 1), j);
+            }
+        }
+        // up to K-1 owned frames and the K-1 behind them
+        for (; q < own + K - 1; q += K) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                if (q + j >= own + K - 1) break;
+                if (q + j < len) {
+                    float g[V];
+                    load_x<T, V, K>(p, q + j, len, b, d, win[(j + K - 1) % K]);
+                    ldv<T, V>(pdo + (p.reverse ? len - 1 - q - j : q + j) * p.do_st, g);
+                    gradient(j, g, q + j < own);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) dp[(j + K - 1) % K][e] = 0.f;
+                }
+                if (q + j - (K - 1) >= s0 || s0 == 0) emit(q + j - (K - 1), j);
+            }
         }
     }
     if (on) {
@@ -212,12 +271,16 @@ __global__ __launch_bounds__(256) void conv_step_kernel(const T* __restrict__ x,
 }
 
 // ---------------------------------------------------------------- C entries
-static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+static bool al(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+static bool al16(const void* p) { return al(p, 16); }
 static bool stride_ok(long long st, int V) { return st % V == 0; }
 
-// frames a thread walks: long enough that the K-1 frames read twice cost little, short enough that the chip is full
-static const int RUN_FWD = 16, RUN_BWD = 32;
-static int run_groups(int T, int run) { return T > 0 ? (T + 4 * run - 1) / (4 * run) : 1; }
+// A thread walks 16 frames forward, 32 backward (rounded up to whole windows): the K-1 frames read twice cost little, and the
+// chip is full.
+static int run_groups(int T, int K, int n) {
+    const int run = 4 * conv_run(K, n);
+    return T > 0 ? (T + run - 1) / run : 1;
+}
 
 #define CONV_K(K_, ...) case K_: { constexpr int K = K_; __VA_ARGS__; break; }
 #define CONV_KS(...) switch (k_) { CONV_K(2, __VA_ARGS__) CONV_K(3, __VA_ARGS__) CONV_K(4, __VA_ARGS__) \
@@ -229,25 +292,26 @@ static int conv_fwd_t(const ConvArgs& p, int k_, hipStream_t stream) {
     constexpr int VW = 16 / sizeof(T);
     const bool vec = p.D % VW == 0 && al16(p.x) && al16(p.out) && al16(p.state) && al16(p.state_out) &&
                      stride_ok(p.x_st, VW) && stride_ok(p.x_sb, VW) && stride_ok(p.o_st, VW) && stride_ok(p.o_sb, VW);
-    const int run = RUN_FWD;
     const int V = vec ? VW : 1;
-    const dim3 grid((p.D + 64 * V - 1) / (64 * V), run_groups(p.T, run), p.B);
-    if (vec) { CONV_KS(hipLaunchKernelGGL((conv_fwd_kernel<T, VW, K>), grid, dim3(256), 0, stream, p, run)) }
-    else { CONV_KS(hipLaunchKernelGGL((conv_fwd_kernel<T, 1, K>), grid, dim3(256), 0, stream, p, run)) }
+    const dim3 grid((p.D + 64 * V - 1) / (64 * V), run_groups(p.T, k_, 16), p.B);
+    if (vec) { CONV_KS(hipLaunchKernelGGL((conv_fwd_kernel<T, VW, K>), grid, dim3(256), 0, stream, p)) }
+    else { CONV_KS(hipLaunchKernelGGL((conv_fwd_kernel<T, 1, K>), grid, dim3(256), 0, stream, p)) }
     ASR_CHECK_LAUNCH();
     return ASR_OK;
 }
+// 8 bytes a thread here: two windows of x and dout on their way, the windows of x and dpre and the parts of dw are 150 registers
+// at 8 bytes, 250 at 16 (one wave per SIMD).  Measured for both passes, 8 / 16 / 4 bytes: T 4096, B 16, D 2048, bf16, K 4: 339 /
+// 398 / 344 us; T 2262, B 16, D 1024, f32: 135 / 139 / 138 us.
 template <typename T>
 static int conv_bwd_t(const ConvArgs& p, int k_, hipStream_t stream) {
-    constexpr int VW = 16 / sizeof(T);
-    const bool vec = p.D % VW == 0 && al16(p.x) && al16(p.dout) && al16(p.state) && al16(p.dstate_out) && al16(p.dx) &&
-                     al16(p.dstate) && stride_ok(p.x_st, VW) && stride_ok(p.x_sb, VW) && stride_ok(p.do_st, VW) &&
+    constexpr int VW = 8 / sizeof(T);
+    const bool vec = p.D % VW == 0 && al(p.x, 8) && al(p.dout, 8) && al(p.state, 8) && al(p.dstate_out, 8) && al(p.dx, 8) &&
+                     al(p.dstate, 8) && stride_ok(p.x_st, VW) && stride_ok(p.x_sb, VW) && stride_ok(p.do_st, VW) &&
                      stride_ok(p.do_sb, VW);
-    const int run = RUN_BWD;
     const int V = vec ? VW : 1;
-    const dim3 grid((p.D + 64 * V - 1) / (64 * V), run_groups(p.T, run), p.B);
-    if (vec) { CONV_KS(hipLaunchKernelGGL((conv_bwd_kernel<T, VW, K>), grid, dim3(256), 0, stream, p, run)) }
-    else { CONV_KS(hipLaunchKernelGGL((conv_bwd_kernel<T, 1, K>), grid, dim3(256), 0, stream, p, run)) }
+    const dim3 grid((p.D + 64 * V - 1) / (64 * V), run_groups(p.T, k_, 32), p.B);
+    if (vec) { CONV_KS(hipLaunchKernelGGL((conv_bwd_kernel<T, VW, K>), grid, dim3(256), 0, stream, p)) }
+    else { CONV_KS(hipLaunchKernelGGL((conv_bwd_kernel<T, 1, K>), grid, dim3(256), 0, stream, p)) }
     ASR_CHECK_LAUNCH();
     return ASR_OK;
 }
@@ -275,7 +339,7 @@ extern "C" int asr_conv_fwd(int dtype, int T, int B, int D, int K, const void* x
 
 extern "C" size_t asr_conv_bwd_ws_bytes(int T, int B, int D, int K) {
     if (T < 0 || B < 0 || D <= 0 || K < 2) return 0;
-    return (size_t)run_groups(T, RUN_BWD) * B * (K + 1) * (size_t)D * sizeof(float);
+    return (size_t)run_groups(T, K, 32) * B * (K + 1) * (size_t)D * sizeof(float);
 }
 
 extern "C" int asr_conv_bwd(int dtype, int T, int B, int D, int K, const void* dout, long long do_st, long long do_sb,
@@ -296,7 +360,7 @@ extern "C" int asr_conv_bwd(int dtype, int T, int B, int D, int K, const void* d
         const int e = dtype == ASR_F32 ? conv_bwd_t<float>(p, K, stream)
                     : dtype == ASR_BF16 ? conv_bwd_t<bf16_t>(p, K, stream) : conv_bwd_t<f16_t>(p, K, stream);
         if (e) return e;
-        P = run_groups(T, RUN_BWD) * B;
+        P = run_groups(T, K, 32) * B;
     }
     sum_partials((const float*)ws, n, P, n, dwb, stream);
     ASR_CHECK_LAUNCH();

@@ -97,10 +97,11 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const T* __restrict__ dy, 
                                                       const float* __restrict__ rstd, const T* __restrict__ dres,
                                                       long long ldd, int rows, int n, T* __restrict__ dx,
                                                       float* __restrict__ part) {
+    constexpr int STEP = 64 * WPR * V, RPB = 4 / WPR;
     __shared__ float sm[4];
+    __shared__ float s_dw[WPR == 1 ? 3 : 1][WPR == 1 ? NV * V * 64 : 1];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int c0 = (WPR == 1 ? lane : (int)threadIdx.x) * V;
-    constexpr int STEP = 64 * WPR * V, RPB = 4 / WPR;
     float dw[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -150,8 +151,18 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const T* __restrict__ dy, 
             stv<T, V>(dx + (size_t)row * n + c, o);
         }
     }
-    // WPR = 1: each of the four waves leaves its own part
-    float* pp = part + ((size_t)blockIdx.x * RPB + (WPR == 1 ? wv : 0)) * n;
+    if constexpr (WPR == 1) {                              // the four waves' parts, joined in order
+        if (wv) {
+#pragma unroll
+            for (int i = 0; i < NV * V; ++i) s_dw[wv - 1][i * 64 + lane] = dw[i / V][i % V];
+        }
+        __syncthreads();
+        if (wv) return;
+#pragma unroll
+        for (int i = 0; i < NV * V; ++i)
+            dw[i / V][i % V] = (dw[i / V][i % V] + s_dw[0][i * 64 + lane]) + (s_dw[1][i * 64 + lane] + s_dw[2][i * 64 + lane]);
+    }
+    float* pp = part + (size_t)blockIdx.x * n;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = c0 + i * STEP;
@@ -205,7 +216,7 @@ static RmsPlan rms_plan(int dtype, int n, bool vec) {
     p.wide = 0;
     return p;
 }
-static const int RMS_BLOCKS = 512;
+static const int RMS_BLOCKS = 1024;
 static int rms_blocks(int rows, int wpr) {
     const int need = (rows + 4 / wpr - 1) / (4 / wpr);
     return need < RMS_BLOCKS ? (need > 0 ? need : 1) : RMS_BLOCKS;
@@ -268,11 +279,10 @@ extern "C" int asr_rms_norm_fwd(int dtype, const void* x, long long ldx, const v
     return ASR_OK;
 }
 
-// the parts of dw: four per workgroup where a wave holds a row (whether it does depends on alignment, so room for four)
+// the parts of dw: one per workgroup, as many as a workgroup per row would need (how many rows share one depends on alignment)
 extern "C" size_t asr_rms_norm_bwd_ws_bytes(int rows, int n) {
     if (rows <= 0 || n <= 0) return 0;
-    const int blocks = rms_blocks(rows, 4);
-    return (size_t)blocks * 4 * n * sizeof(float);
+    return (size_t)rms_blocks(rows, 4) * n * sizeof(float);
 }
 
 extern "C" int asr_rms_norm_bwd(int dtype, const void* dy, long long lddy, const void* x, long long ldx, const void* res,
@@ -288,7 +298,7 @@ extern "C" int asr_rms_norm_bwd(int dtype, const void* dy, long long lddy, const
                          al(dy, 16) && al(x, 16) && al(res, 16) && al(dres, 16) && al(dx, 16) && al(w, 16);
         const RmsPlan pl = rms_plan(dtype, n, vec);
         const int wpr = pl.wide ? pl.wpr : 4, blocks = rms_blocks(rows, wpr);
-        P = blocks * (4 / wpr);
+        P = blocks;
         if (dtype == ASR_F32) rms_bwd_t<float>(pl, blocks, dy, lddy, x, ldx, res, ldr, w, rstd, dres, ldd, rows, n, dx, (float*)ws, stream);
         else if (dtype == ASR_BF16) rms_bwd_t<bf16_t>(pl, blocks, dy, lddy, x, ldx, res, ldr, w, rstd, dres, ldd, rows, n, dx, (float*)ws, stream);
         else rms_bwd_t<f16_t>(pl, blocks, dy, lddy, x, ldx, res, ldr, w, rstd, dres, ldd, rows, n, dx, (float*)ws, stream);

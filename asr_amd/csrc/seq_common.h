@@ -43,13 +43,15 @@ __device__ __forceinline__ float exp_neg_abs_(float v) {
     const float e = __builtin_amdgcn_exp2f(hi);
     return __builtin_fmaf(e, lo * LN2_, e);
 }
-// 1 / (1 + e^-v) from u = e^-|v|: the divisor lies in [1, 2], so a reciprocal and one Newton step serve
+// 1 / (1 + e^-v) from u = e^-|v|, and by itself.  The plain exponent loses |v| 2^-24 of e^-v: of the sigmoid where it is
+// small, of v sigmoid(v) never more than 0.6 * 2^-24 absolute (|v|^2 e^-|v| 2^-24), less than its last rounding near 1.
 __device__ __forceinline__ float sigmoid_from_(float v, float u) {
-    const float d = 1.0f + u, r = __builtin_amdgcn_rcpf(d);
-    const float rr = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
-    return v < 0.0f ? u * rr : rr;
+    const float r = __builtin_amdgcn_rcpf(1.0f + u);
+    return v < 0.0f ? u * r : r;
 }
-__device__ __forceinline__ float sigm_(float v) { return sigmoid_from_(v, exp_neg_abs_(v)); }
+__device__ __forceinline__ float sigm_(float v) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
 __device__ __forceinline__ float silu_(float z) { return z * sigm_(z); }
 // d silu / dz, from z and its sigmoid
 __device__ __forceinline__ float dsilu_(float z, float sg) { return sg * (1.0f + z * (1.0f - sg)); }
@@ -76,19 +78,23 @@ __device__ __forceinline__ int row_len(const int* lens, int b, int T) {
 }
 
 // out[i] = sum over p of part[p * stride + i], i < n, in a fixed order: the second half of every reduction over rows or
-// time.  64 columns x 16 groups of partials per workgroup; a group adds its partials in order, the groups are joined in
-// order in LDS.
+// time.  16 columns x 64 groups of partials per workgroup: few columns and many partials are the usual shape (1024 columns,
+// 2048 partials: 39 us with 64 columns x 16 groups).
 static __global__ __launch_bounds__(1024) void sum_partials_kernel(const float* __restrict__ part, size_t stride, int P,
                                                                    size_t n, float* __restrict__ out) {
-    __shared__ float sm[16][65];
-    const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const size_t i = (size_t)blockIdx.x * 64 + c;
+    __shared__ float sm[16][16];
+    const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const size_t i = (size_t)blockIdx.x * 16 + c;
     float acc = 0.f;
-    if (i < n)
-        for (int p = g; p < P; p += 16) acc += part[(size_t)p * stride + i];
-    sm[g][c] = acc;
+    if (i < n) {
+#pragma unroll 4
+        for (int p = g; p < P; p += 64) acc += part[(size_t)p * stride + i];
+    }
+    acc += __shfl_xor(acc, 16);
+    acc += __shfl_xor(acc, 32);
+    if ((threadIdx.x & 63) < 16) sm[threadIdx.x >> 6][c] = acc;
     __syncthreads();
-    if (g == 0 && i < n) {
+    if (threadIdx.x < 16 && i < n) {
         float t = 0.f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) t += sm[k][c];
@@ -96,8 +102,8 @@ static __global__ __launch_bounds__(1024) void sum_partials_kernel(const float* 
     }
 }
 static inline void sum_partials(const float* part, size_t stride, int P, size_t n, float* out, hipStream_t stream) {
-    if (n) hipLaunchKernelGGL(sum_partials_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, stream, part, stride, P,
-                              n, out);
+    if (n) hipLaunchKernelGGL(sum_partials_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, stream, part, stride, P, n,
+                              out);
 }
 
 static inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
