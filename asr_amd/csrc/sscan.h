@@ -42,8 +42,8 @@ static inline int sscan_nb(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
 static inline int sscan_np(int N) { return 4 * sscan_spl(N) * sscan_nb(N); }
 static inline int sscan_tiles(int T) { return (T + SSCAN_TS - 1) / SSCAN_TS; }
 
-int sscan_chunks(int T, int B, int D, int G);
-int sscan_fill(const asr_sscan_desc* d, SscanArgs* p);
+int sscan_chunks(int T, int B, int D, int G, int backward);
+int sscan_fill(const asr_sscan_desc* d, SscanArgs* p, int backward);
 
 // What a thread of the workgroup knows about its place.
 struct Place {

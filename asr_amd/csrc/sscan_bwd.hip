@@ -36,9 +36,10 @@ __device__ __forceinline__ float sum16(const float (&v)[16], int lane) {
 }
 
 // PRE: the adjoint a chunk hands to the one in front of it when nothing comes in from behind, and its sum of delta.
-// Half way through a tile's adjoints, when half of its states have left their registers, the tile in front of it is called from
-// memory; it goes into the other half of the input buffers behind the last adjoint.  (Called a tile earlier, as the forward
-// pass does, it costs 30 registers where they are scarcest: one wave per SIMD less, or spills.)
+// Behind a tile's first adjoints, when the first of its states have left their registers, the tile in front of it is called from
+// memory; it goes into the other half of the input buffers behind the tile's first barrier, beside the joins.  (Called a tile
+// earlier, as the forward pass does, it costs 30 registers where they are scarcest: one wave per SIMD less, or spills; called
+// half way through the adjoints the spills are 28 registers, and T 2048, B 16, D 2048, bf16 takes 937 us instead of 886.)
 template <typename TY, int SPL, int NB, bool PRE>
 __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanArgs p) {
     constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RS = 8 / SPL;    // RS frames give sixteen sums
@@ -52,6 +53,7 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
     const Place q = sscan_place(p);
     const int tid = threadIdx.x, lane = q.lane, w = q.w;
     if (PRE && (q.k == 0 || q.t0 >= q.t1)) return;
+    // without a gate x stands in for z and the gate's factors are replaced: no branch in the loop
     const bool gated = p.z != nullptr, soft = p.softplus;
     const unsigned d = q.d, off = d * (unsigned)sizeof(TY);
     const float bias = p.bias ? p.bias[d] : 0.f;
@@ -96,7 +98,8 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
         if (!PRE) fetch_rows<FULL>(lx, (const TY*)k->x + q.b * k->x_sb, k->x_st, s0, q.len, rev, off);
         fetch_rows<FULL>(ldt, (const TY*)k->dt + q.b * k->dt_sb, k->dt_st, s0, q.len, rev, off);
         fetch_rows<FULL>(lg, (const TY*)k->dout + q.b * k->do_sb, k->do_st, s0, q.len, rev, off);
-        if (gated) fetch_rows<FULL>(lz, (const TY*)k->z + q.b * k->z_sb, k->z_st, s0, q.len, rev, off);
+        const TY* z = (const TY*)(gated ? k->z : k->x);
+        fetch_rows<FULL>(lz, z + q.b * (gated ? k->z_sb : k->x_sb), gated ? k->z_st : k->x_st, s0, q.len, rev, off);
         if (!PRE) fetch_states<TY, NP, RB>(lB, (const TY*)k->Bm + q.b * k->b_sb + q.g * k->b_sg, k->b_st, tile, q.len, rev, k->N);
         fetch_states<TY, NP, RB>(lC, (const TY*)k->Cm + q.b * k->c_sb + q.g * k->c_sg, k->c_st, tile, q.len, rev, k->N);
     };
@@ -106,19 +109,12 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
         for (int i = 0; i < 4; ++i) {
             const bool ok = FULL || tile * TS + w * 4 + i < q.len;
             const float v = (float)ldt[i] + bias, g = ok ? (float)lg[i] : 0.f;
-            float de = v, dy = g;
-            ns[i] = 1.f;
-            if (soft) {
-                const float u = exp_neg_abs_(v);
-                de = softplus_from_(v, u);
-                ns[i] = sigmoid_from_(v, u);
-            }
-            if (!ok) de = ns[i] = 0.f;
-            if (gated) {
-                const float z = ok ? (float)lz[i] : 0.f, sg = sigm_(z);
-                dy = g * z * sg;
-                ng[i] = g * dsilu_(z, sg);
-            }
+            const float u = exp_neg_abs_(v), sp = softplus_from_(v, u), sv = sigmoid_from_(v, u);
+            const float de = ok ? (soft ? sp : v) : 0.f;
+            ns[i] = ok ? (soft ? sv : 1.f) : 0.f;
+            const float z = ok ? (float)lz[i] : 0.f, sg = sigm_(z);
+            const float dy = gated ? g * z * sg : g;
+            ng[i] = g * dsilu_(z, sg);
             nx[i] = (PRE || !ok) ? 0.f : (float)lx[i];
             s_du[half][w * 4 + i][lane] = float2{de, q.on ? de * nx[i] : 0.f};
             s_dy[half][w * 4 + i][lane] = q.on ? dy : 0.f;
@@ -139,7 +135,7 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
             ck += (size_t)k->D * 4;
         }
     };
-    // a tile; FULL: it and the one in front of it hold valid frames alone, and that is this chunk's too
+    // a tile; FULL: it and the one in front of it hold valid frames alone, and all lanes have a channel
     const auto walk = [&](int tile, auto full) {
         constexpr bool FULL = decltype(full)::value;
         const int half = (q.t1 - 1 - tile) & 1, sb = tile * TS;
@@ -181,7 +177,7 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
                         h[t][j] = __builtin_fmaf(a[t][j], t ? h[t - 1][j] : h0[j], du.y * s_B[half][e]);
                         y = __builtin_fmaf(s_C[half][e], h[t][j], y);
                     }
-                    if (gated) { if (m) s_y[w][t][lane] += y; else s_y[w][t][lane] = y; }
+                    if (m) s_y[w][t][lane] += y; else s_y[w][t][lane] = y;
                 }
 #pragma unroll
                 for (int tb = TS / RS - 1; tb >= 0; --tb) {
@@ -207,7 +203,7 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
                         if (m) { s_s[w][t][lane].x += s1; s_s[w][t][lane].y += s2; }
                         else s_s[w][t][lane] = float2{s1, s2};
                     }
-                    if (m == NB - 1 && tb == TS / RS / 2 && (FULL || tile > q.t0)) {
+                    if (m == NB - 1 && tb == TS / RS - 2 && (FULL || tile > q.t0)) {
                         __builtin_amdgcn_sched_barrier(0);
                         fetch(tile - 1, full);
                         state(tile - 1, 0, hn);
@@ -222,34 +218,31 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
                 for (int j = 0; j < SPL; ++j) dA[m][j] += da[j];
             }
         }
-        // this tile's delta, delta x and dy of the own frames, before their buffers are written again
-        float de[4], dy[4];
-        if (!PRE) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { de[i] = s_du[half][w * 4 + i][lane].x; dy[i] = s_dy[half][w * 4 + i][lane]; }
-        }
-        if (FULL || tile > q.t0) {
-            place(tile - 1, half ^ 1, full);
+        if (PRE) {
+            if (FULL || tile > q.t0) place(tile - 1, half ^ 1, full);
+            __syncthreads();
+            return;
         }
         __syncthreads();
-        if (PRE) return;
+        if (FULL || tile > q.t0) place(tile - 1, half ^ 1, full);      // beside the joins below
         const int s0 = sb + w * 4;
         float ox[4], odt[4], oz[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int t = w * 4 + i;
+            const float de = s_du[half][t][lane].x, dy = s_dy[half][t][lane];
             const float2 a = s_s[0][t][lane], b = s_s[1][t][lane], c = s_s[2][t][lane], e = s_s[3][t][lane];
             const float s1 = (a.x + b.x) + (c.x + e.x), s2 = (a.y + b.y) + (c.y + e.y);
-            ox[i] = __builtin_fmaf(de[i], s1, Dk * dy[i]);
+            ox[i] = __builtin_fmaf(de, s1, Dk * dy);
             odt[i] = __builtin_fmaf(rx[i], s1, s2 * LN2) * rs[i];
-            if (gated) oz[i] = rg[i] * (((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i]);
-            accD = __builtin_fmaf(dy[i], rx[i], accD);     // frames of the padding give zeros
+            oz[i] = rg[i] * (((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i]);
+            accD = __builtin_fmaf(dy, rx[i], accD);     // frames of the padding give zeros
             accb += odt[i];
         }
         const KArgs k = kargs();
         const int T = k->T, rev = k->reverse;
         const long long ost = (long long)k->B * k->D, orow = (long long)q.b * k->D;
-        if (q.on) {
+        if (FULL || q.on) {
             store_rows<FULL>((TY*)k->dx + orow, ost, s0, q.len, T, rev, off, ox);
             store_rows<FULL>((TY*)k->ddt + orow, ost, s0, q.len, T, rev, off, odt);
             if (gated) store_rows<FULL>((TY*)k->dz + orow, ost, s0, q.len, T, rev, off, oz);
@@ -272,7 +265,9 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
     }
     int tile = q.t1 - 1;
     for (; tile >= q.t0 && (tile * TS + TS > q.len); --tile) walk(tile, Flag<false>{});
-    for (; tile >= q.t0 + 1; --tile) walk(tile, Flag<true>{});
+    // (a chunk's first tile calls for the one in front of it, which is thrown away)
+    if (__builtin_amdgcn_ballot_w64(q.on) == ~0ull)
+        for (; tile >= max(q.t0, 1); --tile) walk(tile, Flag<true>{});
     for (; tile >= q.t0; --tile) walk(tile, Flag<false>{});
     if (PRE) {
         if (!q.on) return;
@@ -369,7 +364,7 @@ __global__ __launch_bounds__(256) void sscan_finish_kernel(SscanArgs p, TY* dB, 
 // ---------------------------------------------------------------- C entry
 struct BwdWs { size_t c_h, c_ds, bc, a, d, b, total; };
 static BwdWs bwd_ws(int T, int B, int D, int N, int G) {
-    const int S = sscan_chunks(T, B, D, G), np = sscan_np(N), tpg = (D / G + 63) / 64;
+    const int S = sscan_chunks(T, B, D, G, 1), np = sscan_np(N), tpg = (D / G + 63) / 64;
     BwdWs o{};
     size_t at = 0;
     const auto take = [&](size_t floats) { const size_t v = at; at += align256(floats * 4); return v; };
@@ -407,7 +402,7 @@ static void launch_bwd_t(const SscanArgs& p, const asr_sscan_desc* d, hipStream_
 
 extern "C" int asr_sscan_bwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes, hipStream_t stream) {
     SscanArgs p{};
-    if (int e = sscan_fill(d, &p)) return e;
+    if (int e = sscan_fill(d, &p, 1)) return e;
     if (!d->dA || (d->z && !d->dz && d->T > 0 && d->B > 0)) return ASR_ERR_ARG;
     if (d->T > 0 && d->B > 0 && (!d->dout || !d->ckpt || !d->dx || !d->ddt || !d->dB || !d->dC)) return ASR_ERR_ARG;
     if (d->dh0 && d->dh0 == d->dh_last) return ASR_ERR_ARG;

@@ -17,7 +17,10 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
     if (PRE && q.t0 >= q.t1) return;
     const TY* px = (const TY*)p.x + q.b * p.x_sb;
     const TY* pdt = (const TY*)p.dt + q.b * p.dt_sb;
-    const TY* pz = p.z ? (const TY*)p.z + q.b * p.z_sb : nullptr;
+    // without a gate the input stands in for z and the gate's factor is replaced by 1: no branch in the loop
+    const bool gated = p.z != nullptr, soft = p.softplus;
+    const TY* pz = gated ? (const TY*)p.z + q.b * p.z_sb : px;
+    const long long z_st = gated ? p.z_st : p.x_st;
     const TY* pB = (const TY*)p.Bm + q.b * p.b_sb + q.g * p.b_sg;
     const TY* pC = (const TY*)p.Cm + q.b * p.c_sb + q.g * p.c_sg;
     TY* po = (TY*)p.out + q.b * p.o_sb;
@@ -56,7 +59,7 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
         const int s0 = tile * TS + w * 4;
         fetch_rows<FULL>(lx, px, p.x_st, s0, q.len, p.reverse, off);
         fetch_rows<FULL>(ldt, pdt, p.dt_st, s0, q.len, p.reverse, off);
-        if (!PRE && pz) fetch_rows<FULL>(lz, pz, p.z_st, s0, q.len, p.reverse, off);
+        if (!PRE) fetch_rows<FULL>(lz, pz, z_st, s0, q.len, p.reverse, off);
         fetch_states<TY, NP, RB>(lB, pB, p.b_st, tile, q.len, p.reverse, p.N);
         if (!PRE) fetch_states<TY, NP, RB>(lC, pC, p.c_st, tile, q.len, p.reverse, p.N);
     };
@@ -66,10 +69,10 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
         for (int i = 0; i < 4; ++i) {
             const bool ok = FULL || tile * TS + w * 4 + i < q.len;
             const float v = (float)ldt[i] + bias;
-            const float sp = p.softplus ? softplus_(v) : v;
-            const float de = ok ? sp : 0.f;
+            const float sp = softplus_(v), raw = soft ? sp : v;
+            const float de = ok ? raw : 0.f;
             nx[i] = ok ? (float)lx[i] : 0.f;
-            nz[i] = (!PRE && pz) ? (float)lz[i] : 0.f;
+            if (!PRE) nz[i] = (float)lz[i];
             s_du[half][w * 4 + i][lane] = float2{de, de * nx[i]};
         }
         place_states<TY, NP, RB>(s_B[half], lB, tile, q.len, p.N);
@@ -77,25 +80,36 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
     };
     float* ck = (!PRE && p.ckpt) ? p.ckpt + (((size_t)q.t0 * p.B + q.b) * NP + w * SPL) * p.D : nullptr;
     const size_t ck_tile = (size_t)p.B * NP * p.D;
-    // a tile; FULL: it, the next and the one after that hold valid frames alone
-    const auto walk = [&](int tile, auto full) {
+    // what a tile leaves behind: y joined, gated, stored
+    const auto leave = [&](int tile, int half, auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = w * 4 + i;
+            y[i] = ((s_y[half][0][t][lane] + s_y[half][1][t][lane]) + (s_y[half][2][t][lane] + s_y[half][3][t][lane])) + Dk * rx[i];
+            y[i] *= gated ? silu_(rz[i]) : 1.0f;
+        }
+        if (FULL || q.on) store_rows<FULL>(po, p.o_st, tile * TS + w * 4, q.len, p.T, p.reverse, off, y);
+    };
+    // a tile, and behind it the tile in front (`prev`), so that its joins and stores run beside the walk.  FULL: it, the next
+    // and the one after that, and the one in front, hold valid frames alone, and all lanes have a channel
+    const auto walk = [&](int tile, auto full, auto prev) {
         constexpr bool FULL = decltype(full)::value;
         const int half = (tile - q.t0) & 1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { rx[i] = nx[i]; rz[i] = nz[i]; }
         if (!PRE && ck) {
-            unsigned at = d * 4u;
-            if (q.on)
+            if (FULL || q.on)
 #pragma unroll
                 for (int m = 0; m < NB; ++m)
 #pragma unroll
-                    for (int j = 0; j < SPL; ++j) {
-                        char* r = (char*)(ck + (size_t)(m * 4 * SPL + j) * p.D);
-                        *(float*)(r + at) = h[m][j];
-                    }
+                    for (int j = 0; j < SPL; ++j)
+                        *(float*)((char*)(ck + (size_t)(m * 4 * SPL + j) * p.D) + d * 4u) = h[m][j];
             ck += ck_tile;
         }
+        if (!PRE && decltype(prev)::value) leave(tile - 1, half ^ 1, full);
 #pragma unroll
+        for (int i = 0; i < 4; ++i) { rx[i] = nx[i]; rz[i] = nz[i]; }
+#pragma unroll(NB == 1 ? TS : 4)
         for (int t = 0; t < TS; ++t) {
             const float2 du = s_du[half][t][lane];
             float y = 0.f;
@@ -115,17 +129,6 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
             fetch(FULL ? tile + 2 : min(tile + 2, q.t1 - 1), full);
         }
         __syncthreads();
-        if (!PRE && q.on) {
-            float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = w * 4 + i;
-                y[i] = ((s_y[half][0][t][lane] + s_y[half][1][t][lane]) +
-                        (s_y[half][2][t][lane] + s_y[half][3][t][lane])) + Dk * rx[i];
-                if (pz) y[i] *= silu_(rz[i]);
-            }
-            store_rows<FULL>(po, p.o_st, tile * TS + w * 4, q.len, p.T, p.reverse, off, y);
-        }
     };
     if (q.t0 < q.t1) {
         fetch(q.t0, Flag<false>{});
@@ -133,10 +136,14 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
         fetch(min(q.t0 + 1, q.t1 - 1), Flag<false>{});
         __syncthreads();
     }
-    const int clear = min(q.t1, q.len / TS) - 2;
+    // (a chunk's last tiles call for the next chunk's first two: valid frames, thrown away)
+    const int clear = __builtin_amdgcn_ballot_w64(q.on) == ~0ull ? min(q.t1, q.len / TS - 2) : 0;
     int tile = q.t0;
-    for (; tile < clear; ++tile) walk(tile, Flag<true>{});
-    for (; tile < q.t1; ++tile) walk(tile, Flag<false>{});
+    if (tile < clear) walk(tile++, Flag<true>{}, Flag<false>{});
+    else if (tile < q.t1) walk(tile++, Flag<false>{}, Flag<false>{});
+    for (; tile < clear; ++tile) walk(tile, Flag<true>{}, Flag<true>{});
+    for (; tile < q.t1; ++tile) walk(tile, Flag<false>{}, Flag<true>{});
+    if (!PRE && q.t0 < q.t1) leave(q.t1 - 1, (q.t1 - 1 - q.t0) & 1, Flag<false>{});
     if (!q.on) return;
     if (PRE) {
 #pragma unroll
@@ -205,21 +212,22 @@ __global__ __launch_bounds__(256) void sscan_step_kernel(SscanArgs p) {
 }
 
 // ---------------------------------------------------------------- C entries
-// Chunks of time.  One while batch rows x channel tiles give every CU two workgroups (512; the two waves per SIMD that the
-// backward pass has registers for): a second pass over the chunks then only costs (T 2048, B 16, D 2048, bf16, 512 workgroups:
-// forward 379 us with one chunk, 482 with two; backward 1043, 1249).  With fewer, as many chunks as make 1024 workgroups (T 1207,
-// B 16, D 1024, f32, ragged, 256 workgroups: 1 / 2 / 4 chunks: forward 184 / 173 / 161 us, backward 487 / 391 / 363; T 16384,
-// B 1, D 2048, bf16, 32 workgroups: 8 / 16 / 32 / 64 chunks: forward 453 / 310 / 287 / 286 us), of at least four tiles each.
-int sscan_chunks(int T, int B, int D, int G) {
+// Chunks of time.  One while batch rows x channel tiles give every CU two workgroups (512): a second pass over the chunks then
+// only costs (T 2048, B 16, D 2048, bf16, 512 workgroups: forward 379 us with one chunk, 482 with two; backward 1043, 1249).
+// With fewer, forward as many chunks as fill the three workgroups that a CU's LDS holds (768), backward 1024, two rounds of the
+// two it holds, which evens out ragged rows (T 1207, B 16, D 1024, f32, ragged, 256 workgroups: 1 / 2 / 3 / 4 chunks: forward 184 /
+// 173 / 155 / 161 us, backward 487 / 391 / 394 / 363; T 16384, B 1, D 2048, bf16, 32 workgroups, forward: 8 / 16 / 24 / 32 / 64
+// chunks: 453 / 310 / 277 / 287 / 286 us), of at least four tiles each.
+int sscan_chunks(int T, int B, int D, int G, int backward) {
     const long long wgs = (long long)G * ((D / G + 63) / 64) * B;
     const int nt = sscan_tiles(T);
-    long long S = wgs > 0 && wgs < 512 ? 1024 / wgs : 1;
+    long long S = wgs > 0 && wgs < 512 ? (backward ? 1024 : 768) / wgs : 1;
     if (S > nt / 4) S = nt / 4;
     if (S > 64) S = 64;
     return S < 1 ? 1 : (int)S;
 }
 
-int sscan_fill(const asr_sscan_desc* d, SscanArgs* p) {
+int sscan_fill(const asr_sscan_desc* d, SscanArgs* p, int backward) {
     if (!d || d->dtype < ASR_F32 || d->dtype > ASR_F16) return ASR_ERR_ARG;
     if (d->T < 0 || d->B < 0 || d->D <= 0 || d->N <= 0 || d->G <= 0 || d->D % d->G) return ASR_ERR_ARG;
     if (d->N > 64 || d->B > 65535 || d->D > (1 << 24) || d->T > (1 << 24)) return ASR_ERR_LIMIT;
@@ -229,7 +237,7 @@ int sscan_fill(const asr_sscan_desc* d, SscanArgs* p) {
     p->T = d->T; p->B = d->B; p->D = d->D; p->N = d->N; p->G = d->G;
     p->dpg = d->D / d->G; p->tpg = (p->dpg + 63) / 64;
     p->reverse = d->reverse; p->softplus = d->softplus;
-    p->S = sscan_chunks(d->T, d->B, d->D, d->G);
+    p->S = sscan_chunks(d->T, d->B, d->D, d->G, backward);
     p->tpc = (sscan_tiles(d->T) + p->S - 1) / p->S;
     if (p->tpc < 1) p->tpc = 1;
     p->np = sscan_np(d->N);
@@ -253,7 +261,7 @@ extern "C" size_t asr_sscan_ckpt_floats(int T, int B, int D, int N) {
 }
 
 static size_t fwd_ws(int T, int B, int D, int N, int G) {
-    const int S = sscan_chunks(T, B, D, G);
+    const int S = sscan_chunks(T, B, D, G, 0);
     return S > 1 ? align256((size_t)S * B * sscan_np(N) * D * 4) + (size_t)S * B * D * 4 : 0;
 }
 
@@ -280,7 +288,7 @@ static void launch_fwd_t(const SscanArgs& p, hipStream_t stream) {
 
 extern "C" int asr_sscan_fwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes, hipStream_t stream) {
     SscanArgs p{};
-    if (int e = sscan_fill(d, &p)) return e;
+    if (int e = sscan_fill(d, &p, 0)) return e;
     if (d->h_last && d->h_last == d->h0) return ASR_ERR_ARG;
     if (d->T > 0 && d->B > 0 && !d->out) return ASR_ERR_ARG;
     if (d->B == 0 || (d->T == 0 && !d->h_last)) return ASR_OK;
