@@ -214,14 +214,14 @@ __global__ __launch_bounds__(256) void sscan_step_kernel(SscanArgs p) {
 // ---------------------------------------------------------------- C entries
 // Chunks of time.  One while batch rows x channel tiles give every CU two workgroups (512): a second pass over the chunks then
 // only costs (T 2048, B 16, D 2048, bf16, 512 workgroups: forward 379 us with one chunk, 482 with two; backward 1043, 1249).
-// With fewer, forward as many chunks as fill the three workgroups that a CU's LDS holds (768), backward 1024, two rounds of the
-// two it holds, which evens out ragged rows (T 1207, B 16, D 1024, f32, ragged, 256 workgroups: 1 / 2 / 3 / 4 chunks: forward 184 /
-// 173 / 155 / 161 us, backward 487 / 391 / 394 / 363; T 16384, B 1, D 2048, bf16, 32 workgroups, forward: 8 / 16 / 24 / 32 / 64
-// chunks: 453 / 310 / 277 / 287 / 286 us), of at least four tiles each.
+// With fewer, forward as many chunks as fill the three workgroups that a CU's LDS holds (768; T 1207, B 16, D 1024, f32, ragged, 256
+// workgroups: 2 / 3 / 4 / 6 / 8 chunks: 183 / 151 / 155 / 153 / 148 us; T 16384, B 1, D 2048, bf16, 32 workgroups: 8 / 16 / 24 / 32 /
+// 64 chunks: 453 / 310 / 277 / 287 / 286 us), backward four rounds of the two it holds (2048), which evens out ragged rows (the
+// first case: 4 / 6 / 8 / 10 / 12 chunks: 315 / 308 / 294 / 310 / 309 us), of at least four tiles each.
 int sscan_chunks(int T, int B, int D, int G, int backward) {
     const long long wgs = (long long)G * ((D / G + 63) / 64) * B;
     const int nt = sscan_tiles(T);
-    long long S = wgs > 0 && wgs < 512 ? (backward ? 1024 : 768) / wgs : 1;
+    long long S = wgs > 0 && wgs < 512 ? (backward ? 2048 : 768) / wgs : 1;
     if (S > nt / 4) S = nt / 4;
     if (S > 64) S = 64;
     return S < 1 ? 1 : (int)S;

@@ -34,6 +34,11 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _new(t, _row_major=torch.contiguous_format):
+    """a contiguous tensor of t's shape and type (None for None)"""
+    return None if t is None else torch.empty_like(t, memory_format=_row_major)
+
+
 def _act(name, t, shape, dtype, dev):
     """an activation: the shape, the call's type, the call's device, unit stride of the last axis; -> its strides"""
     st = t.stride()
@@ -131,7 +136,7 @@ def causal_conv_fwd(x, w, bias=None, state=None, lens=None, act='silu', reverse=
     if want_state, else None)."""
     kind, T, B, D, K, dev, st, pw, pb, ps, pl, silu = _conv_args(x, w, bias, state, lens, act)
     _gpu(dev)
-    out = torch.empty((T, B, D), dtype=x.dtype, device=x.device)
+    out = _new(x)
     new = torch.empty((K - 1, B, D), dtype=x.dtype, device=x.device) if want_state else None
     _call('asr_conv_fwd', dev, _lib.lib().asr_conv_fwd, kind, T, B, D, K, x.data_ptr(), st[0], st[1], pw, pb, ps, pl, silu,
           int(reverse), out.data_ptr(), B * D, D, _p(new))
@@ -146,7 +151,7 @@ def causal_conv_bwd(dout, x, w, bias=None, state=None, lens=None, act='silu', re
     pd = _par('dstate_out', dstate_out, (K - 1, B, D), dev, x.dtype) if dstate_out is not None else None
     _gpu(dev)
     L = _lib.lib()
-    dx = torch.empty((T, B, D), dtype=x.dtype, device=x.device)
+    dx = _new(x)
     dwb = torch.empty(D * (K + 1), dtype=torch.float32, device=x.device)
     ds = torch.empty((K - 1, B, D), dtype=x.dtype, device=x.device) if state is not None else None
     need = L.asr_conv_bwd_ws_bytes(T, B, D, K)
@@ -174,7 +179,7 @@ def causal_conv_step(x, state, w, bias=None, act='silu'):
     ps = _par('state', state, (K - 1, B, D), dev, ty)
     silu = _act_kind(act)
     _gpu(dev)
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    out = _new(x)
     _call('asr_conv_step', dev, _lib.lib().asr_conv_step, kind, B, D, K, x.data_ptr(), st[0], ps, pw, pb, silu, out.data_ptr(), D)
     return out
 
@@ -225,7 +230,7 @@ def selective_scan_fwd(x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, h0=None, 
     _gpu(dev)
     L = _lib.lib()
     f32, on = torch.float32, x.device
-    out = torch.empty((T, B, Dn), dtype=x.dtype, device=on)
+    out = _new(x)
     h = torch.empty((B, Dn, N), dtype=f32, device=on)
     saved = torch.empty(L.asr_sscan_ckpt_floats(T, B, Dn, N), dtype=f32, device=on) if train else None
     need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 0)
@@ -248,14 +253,9 @@ def selective_scan_bwd(dout, x, dt, A, Bm, Cm, saved, D=None, z=None, dt_bias=No
     ps = _par('saved', saved, saved.shape, dev)
     ph = _par('dh_last', dh_last, (B, Dn, N), dev) if dh_last is not None else None
     _gpu(dev)
-    ty, f32, on = x.dtype, torch.float32, x.device
-    wide, states = (T, B, Dn), (T, B, G, N)
-    g = {'x': torch.empty(wide, dtype=ty, device=on), 'dt': torch.empty(wide, dtype=ty, device=on),
-         'A': torch.empty((Dn, N), dtype=f32, device=on), 'B': torch.empty(states, dtype=ty, device=on),
-         'C': torch.empty(states, dtype=ty, device=on), 'D': torch.empty_like(D) if D is not None else None,
-         'z': torch.empty(wide, dtype=ty, device=on) if z is not None else None,
-         'dt_bias': torch.empty_like(dt_bias) if dt_bias is not None else None,
-         'h0': torch.empty_like(h0) if h0 is not None else None}
+    on = x.device
+    g = {'x': _new(x), 'dt': _new(dt), 'A': _new(A), 'B': _new(Bm), 'C': _new(Cm), 'D': _new(D), 'z': _new(z),
+         'dt_bias': _new(dt_bias), 'h0': _new(h0)}
     need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 1)
     ws = torch.empty(need, dtype=torch.uint8, device=on)
     desc = _lib.SscanDesc(*members, None, 0, 0, None, ps, dout.data_ptr(), so[0], so[1], ph, g['x'].data_ptr(),
@@ -282,7 +282,7 @@ def selective_scan_step(h, x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, softp
     pb = _par('dt_bias', dt_bias, (Dn,), dev) if dt_bias is not None else None
     ph = _par('h', h, (B, Dn, N), dev)
     _gpu(dev)
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    out = _new(x)
     _call('asr_sscan_step', dev, _lib.lib().asr_sscan_step, kind, B, Dn, N, G, ph, x.data_ptr(), sx[0], dt.data_ptr(), sd[0], pA,
           Bm.data_ptr(), sB[0], sB[1], Cm.data_ptr(), sC[0], sC[1], pD, pz, sz, pb, 1 if softplus else 0, out.data_ptr(), Dn)
     return out
@@ -308,8 +308,8 @@ def add_rms_norm_fwd(x, w, residual=None, eps=1e-6):
     if not eps >= 0:
         _fail('eps: %r is negative' % (eps,))
     _gpu(dev)
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    r = torch.empty_like(y) if pr is not None else None
+    y = _new(x)
+    r = _new(residual)
     rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
     _call('asr_rms_norm_fwd', dev, _lib.lib().asr_rms_norm_fwd, kind, x.data_ptr(), sx[0], pr, sr, pw, rows, n, eps,
           y.data_ptr(), _p(r), rstd.data_ptr())
@@ -329,8 +329,7 @@ def add_rms_norm_bwd(dy, x, w, rstd, residual=None, dres=None):
     pd, sd = (dres.data_ptr(), _act('dres', dres, sh, ty, dev)[0]) if dres is not None else (None, 0)
     _gpu(dev)
     L = _lib.lib()
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    dw = torch.empty_like(w)
+    dx, dw = _new(x), _new(w)
     need = L.asr_rms_norm_bwd_ws_bytes(rows, n)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _call('asr_rms_norm_bwd', dev, L.asr_rms_norm_bwd, kind, dy.data_ptr(), sy[0], x.data_ptr(), sx[0], pr, sr, pw, ps, pd, sd,
@@ -362,10 +361,11 @@ def clip_list(tensors, max_norm, eps=1e-7):
         mine = [i for i in range(n) if kinds[i] == kind]
         if not mine:
             continue
-        flat = torch.empty(sum([sizes[i] for i in mine]), dtype=dtype, device=on)
+        parts = [sizes[i] for i in mine]
+        flat = torch.empty(sum(parts), dtype=dtype, device=on)
         at, e = flat.data_ptr(), flat.element_size()
-        for i, view in zip(mine, torch._C._nn.unflatten_dense_tensors(flat, [src[i] for i in mine])):
-            out[i], dst[i] = view, at
+        for i, view in zip(mine, flat.split(parts)):
+            out[i], dst[i] = (view if src[i].dim() == 1 else view.view(src[i].shape)), at
             at += sizes[i] * e
     L = _lib.lib()
     csizes = (C.c_longlong * n)(*sizes)
