@@ -124,7 +124,7 @@ def test_training_step_of_a_block(reverse):
     rx = R.leaf(x)
     rl = ref_loss(rp, rx, R.leaf(res, False), y.cpu(), mask.cpu().double(), lens_l, reverse)
     rl.backward()
-    assert abs(float(loss) - float(rl)) < 2000 * R.U * abs(float(rl))
+    assert abs(float(loss) - rl.item()) < 2000 * R.U * abs(rl.item())
     R.close(dx, rx.grad, 2000, 'dx')
     assert sorted(grads) == sorted(p)
     for k in p:
@@ -141,7 +141,7 @@ def test_training_step_of_a_block(reverse):
         rp[k].data -= lr * v.cpu().double()
     new = ref_loss(rp, rx, R.leaf(res, False), y.cpu(), mask.cpu().double(), lens_l, reverse)
     want = lr * 0.5 * float(rnorm)
-    assert 0.9 * want < float(rl) - float(new) < 1.1 * want
+    assert 0.9 * want < rl.item() - new.item() < 1.1 * want
 
 
 def test_streaming_of_a_block():
