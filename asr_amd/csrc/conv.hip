@@ -327,7 +327,8 @@ static int conv_bwd_t(const ConvArgs& p, int k_, hipStream_t stream) {
 
 static int conv_dims_ok(int dtype, int T, int B, int D, int K) {
     if (dtype < ASR_F32 || dtype > ASR_F16 || T < 0 || B < 0 || D <= 0 || K < 2) return ASR_ERR_ARG;
-    if (K > 8 || B > 65535 || D > (1 << 24) || T > (1 << 21)) return ASR_ERR_LIMIT;   // grid axes y, z end at 65535
+    // grid axes y and z end at 65535, a launch at 2^32 work items
+    if (K > 8 || B > 65535 || D > (1 << 20) || T > (1 << 21)) return ASR_ERR_LIMIT;
     return ASR_OK;
 }
 
@@ -360,6 +361,7 @@ extern "C" int asr_conv_bwd(int dtype, int T, int B, int D, int K, const void* d
     const size_t n = (size_t)D * (K + 1);
     if (T && B && (!x || !dout || !dx)) return ASR_ERR_ARG;
     if (ws_bytes < asr_conv_bwd_ws_bytes(T, B, D, K) || (B && !ws)) return ASR_ERR_WS;
+    if ((uintptr_t)ws & 15) return ASR_ERR_ARG;
     int P = 0;
     if (B) {
         ConvArgs p{};
@@ -394,6 +396,7 @@ static int conv_step_t(int B, int D, int k_, const void* x, long long x_sb, void
 extern "C" int asr_conv_step(int dtype, int B, int D, int K, const void* x, long long x_sb, void* state, const float* w,
                              const float* bias, int act, void* out, long long o_sb, hipStream_t stream) {
     if (int e = conv_dims_ok(dtype, 1, B, D, K)) return e;
+    if ((long long)B * D > (1ll << 31)) return ASR_ERR_LIMIT;
     if (!w) return ASR_ERR_ARG;
     if (!B) return ASR_OK;
     if (!x || !state || !out) return ASR_ERR_ARG;

@@ -128,9 +128,9 @@ extern "C" int asr_clip_list(int count, const int* dtypes, const void* const* sr
         if (sizes[i] > (1ll << 40)) return ASR_ERR_LIMIT;
         total += chunks_of(sizes[i]);
     }
-    if (total > 0x7fffffff) return ASR_ERR_LIMIT;
+    if (total >= (1 << 24)) return ASR_ERR_LIMIT;                // 2^32 work items a launch
     if (!ws || ws_bytes < asr_clip_list_ws_bytes(count, sizes)) return ASR_ERR_WS;
-    if ((uintptr_t)ws & 7) return ASR_ERR_ARG;
+    if ((uintptr_t)ws & 15) return ASR_ERR_ARG;
     double* part = (double*)ws;
     float* mult = (float*)(part + total);
     for (int pass = 0; pass < 2; ++pass) {

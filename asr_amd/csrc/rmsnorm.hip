@@ -266,7 +266,7 @@ static void rms_bwd_t(const RmsPlan& pl, int blocks, const void* dy, long long l
 extern "C" int asr_rms_norm_fwd(int dtype, const void* x, long long ldx, const void* res, long long ldr, const float* w,
                                 int rows, int n, float eps, void* y, void* sum, float* rstd, hipStream_t stream) {
     if (dtype < ASR_F32 || dtype > ASR_F16 || rows < 0 || n <= 0 || !w || !(eps >= 0.f)) return ASR_ERR_ARG;
-    if (rows > (1 << 30) || n > (1 << 28)) return ASR_ERR_LIMIT;
+    if (rows >= (1 << 24) || n > (1 << 25)) return ASR_ERR_LIMIT;       // 2^32 work items a launch
     if (rows == 0) return ASR_OK;
     if (!x || !y) return ASR_ERR_ARG;
     const int e = (int)elem_size(dtype), V = 16 / e;
@@ -290,9 +290,10 @@ extern "C" int asr_rms_norm_bwd(int dtype, const void* dy, long long lddy, const
                                 long long ldr, const float* w, const float* rstd, const void* dres, long long ldd, int rows, int n, void* dx, float* dw,
                                 void* ws, size_t ws_bytes, hipStream_t stream) {
     if (dtype < ASR_F32 || dtype > ASR_F16 || rows < 0 || n <= 0 || !w || !dw) return ASR_ERR_ARG;
-    if (rows > (1 << 30) || n > (1 << 28)) return ASR_ERR_LIMIT;
+    if (rows >= (1 << 24) || n > (1 << 25)) return ASR_ERR_LIMIT;       // 2^32 work items a launch
     if (rows && (!dy || !x || !rstd || !dx)) return ASR_ERR_ARG;
     if (rows && (!ws || ws_bytes < asr_rms_norm_bwd_ws_bytes(rows, n))) return ASR_ERR_WS;
+    if ((uintptr_t)ws & 15) return ASR_ERR_ARG;
     int P = 0;
     if (rows) {
         const int V = 16 / (int)elem_size(dtype);

@@ -82,7 +82,8 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
                 }
         }
     }
-    if (!q.on) {                                // idle lanes stand on a real channel: they must give nothing to dB and dC
+    // idle lanes stand on a real channel: whatever it holds, they must give zeros to the sums dB and dC
+    if (!q.on) {
 #pragma unroll
         for (int m = 0; m < NB; ++m)
 #pragma unroll
@@ -110,14 +111,15 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
             const bool ok = FULL || tile * TS + w * 4 + i < q.len;
             const float v = (float)ldt[i] + bias, g = ok ? (float)lg[i] : 0.f;
             const float u = exp_neg_abs_(v), sp = softplus_from_(v, u), sv = sigmoid_from_(v, u);
-            const float de = ok ? (soft ? sp : v) : 0.f;
+            const bool live = ok && (FULL || q.on);
+            const float de = live ? (soft ? sp : v) : 0.f;
             ns[i] = ok ? (soft ? sv : 1.f) : 0.f;
             const float z = ok ? (float)lz[i] : 0.f, sg = sigm_(z);
             const float dy = gated ? g * z * sg : g;
             ng[i] = g * dsilu_(z, sg);
             nx[i] = (PRE || !ok) ? 0.f : (float)lx[i];
-            s_du[half][w * 4 + i][lane] = float2{de, q.on ? de * nx[i] : 0.f};
-            s_dy[half][w * 4 + i][lane] = q.on ? dy : 0.f;
+            s_du[half][w * 4 + i][lane] = float2{de, live ? de * nx[i] : 0.f};
+            s_dy[half][w * 4 + i][lane] = live ? dy : 0.f;
         }
         const int N = kargs()->N;
         if (!PRE) place_states<TY, NP, RB>(s_B[half], lB, tile, q.len, N);
@@ -131,7 +133,7 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
         unsigned at = d * 4u;
 #pragma unroll
         for (int j = 0; j < SPL; ++j) {
-            o[j] = *(const float*)(ck + at);
+            o[j] = q.on ? *(const float*)(ck + at) : 0.f;
             ck += (size_t)k->D * 4;
         }
     };
@@ -406,9 +408,10 @@ extern "C" int asr_sscan_bwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes,
     if (!d->dA || (d->z && !d->dz && d->T > 0 && d->B > 0)) return ASR_ERR_ARG;
     if (d->T > 0 && d->B > 0 && (!d->dout || !d->ckpt || !d->dx || !d->ddt || !d->dB || !d->dC)) return ASR_ERR_ARG;
     if (d->dh0 && d->dh0 == d->dh_last) return ASR_ERR_ARG;
-    if ((double)d->B * d->T * 2 * p.np * d->G > 256.0 * 0x7fff0000) return ASR_ERR_LIMIT;        // blocks of a launch
+    if ((double)d->B * d->T * 2 * p.np * d->G > 4.0e9) return ASR_ERR_LIMIT;        // one work item each, 2^32 a launch
     const BwdWs o = bwd_ws(d->T, d->B, d->D, d->N, d->G);
     if (o.total && (!ws || ws_bytes < o.total)) return ASR_ERR_WS;
+    if ((uintptr_t)ws & 15) return ASR_ERR_ARG;
     char* base = (char*)ws;
     p.c_h = (float*)(base + o.c_h); p.c_ds = (float*)(base + o.c_ds); p.part_bc = (float*)(base + o.bc);
     p.part_a = (float*)(base + o.a); p.part_d = (float*)(base + o.d); p.part_b = (float*)(base + o.b);

@@ -230,7 +230,7 @@ int sscan_chunks(int T, int B, int D, int G, int backward) {
 int sscan_fill(const asr_sscan_desc* d, SscanArgs* p, int backward) {
     if (!d || d->dtype < ASR_F32 || d->dtype > ASR_F16) return ASR_ERR_ARG;
     if (d->T < 0 || d->B < 0 || d->D <= 0 || d->N <= 0 || d->G <= 0 || d->D % d->G) return ASR_ERR_ARG;
-    if (d->N > 64 || d->B > 65535 || d->D > (1 << 24) || d->T > (1 << 24)) return ASR_ERR_LIMIT;
+    if (d->N > 64 || d->B > 65535 || d->D > (1 << 20) || d->T > (1 << 24)) return ASR_ERR_LIMIT;
     if (!d->A) return ASR_ERR_ARG;
     const bool any = d->T > 0 && d->B > 0;
     if (any && (!d->x || !d->dt || !d->Bm || !d->Cm)) return ASR_ERR_ARG;
@@ -294,6 +294,7 @@ extern "C" int asr_sscan_fwd(const asr_sscan_desc* d, void* ws, size_t ws_bytes,
     if (d->B == 0 || (d->T == 0 && !d->h_last)) return ASR_OK;
     if (p.S > 1) {
         if (!ws || ws_bytes < fwd_ws(d->T, d->B, d->D, d->N, d->G)) return ASR_ERR_WS;
+        if ((uintptr_t)ws & 15) return ASR_ERR_ARG;
         p.c_h = (float*)ws;
         p.c_ds = (float*)((char*)ws + align256((size_t)p.S * p.B * p.np * p.D * 4));
     }
@@ -321,7 +322,8 @@ extern "C" int asr_sscan_step(int dtype, int B, int D, int N, int G, float* h, c
                               long long z_sb, const float* dt_bias, int softplus, void* out, long long o_sb,
                               hipStream_t stream) {
     if (dtype < ASR_F32 || dtype > ASR_F16 || B < 0 || D <= 0 || N <= 0 || G <= 0 || D % G || !A) return ASR_ERR_ARG;
-    if (N > 64 || B > 65535 || D > (1 << 24)) return ASR_ERR_LIMIT;
+    // 2^32 work items a launch: up to 16 of them a channel
+    if (N > 64 || B > 65535 || D > (1 << 20) || (long long)B * D > (1ll << 27)) return ASR_ERR_LIMIT;
     if (!B) return ASR_OK;
     if (!h || !x || !dt || !Bm || !Cm || !out) return ASR_ERR_ARG;
     SscanArgs p{};

@@ -27,7 +27,8 @@ def _fail(msg):
     raise ValueError(msg)
 
 
-_stream = torch._C._cuda_getCurrentRawStream          # the handle alone: torch.cuda.current_stream() makes an object of it
+# the handle alone: torch.cuda.current_stream() makes an object of it
+_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _p(t):

@@ -185,6 +185,16 @@ def test_c_entries_refuse_before_they_launch():
     assert L.asr_clip_list(1, kind, ptr, ptr, (C.c_longlong * 1)(-1), 1.0, 1e-7, p, p, need, None) == ARG
     assert L.asr_clip_list(1, kind, (C.c_void_p * 1)(None), ptr, one, 1.0, 1e-7, p, p, need, None) == ARG
     assert L.asr_clip_list(1, kind, ptr, ptr, one, 1.0, 1e-7, p, p + 4, need, None) == ARG
+    # beyond a launch's work items, and workspaces off the 16-byte grid
+    assert L.asr_sscan_bwd(desc(T=1 << 23, B=64), p, 1 << 60, None) == LIMIT
+    assert L.asr_sscan_step(0, 1 << 13, 1 << 15, 16, 1, p, p, 8, p, 8, p, p, 16, 16, p, 16, 16, None, None, 0, None, 1, p, 8, None) == LIMIT
+    assert L.asr_rms_norm_fwd(0, p, 8, None, 0, p, 1 << 24, 8, 1e-6, p, None, None, None) == LIMIT
+    assert L.asr_clip_list(1, kind, ptr, ptr, (C.c_longlong * 1)(1 << 38), 1.0, 1e-7, p, p, 1 << 60, None) == LIMIT
+    assert L.asr_conv_fwd(0, 1 << 22, 2, 8, 4, p, 16, 8, p, None, None, None, 1, 0, p, 16, 8, None, None) == LIMIT
+    assert L.asr_conv_fwd(0, 4, 2, 1 << 21, 4, p, 16, 8, p, None, None, None, 1, 0, p, 16, 8, None, None) == LIMIT
+    assert L.asr_sscan_fwd(desc(), p + 8, 1 << 40, None) == ARG and L.asr_sscan_bwd(desc(), p + 8, 1 << 40, None) == ARG
+    assert L.asr_conv_bwd(0, 30, 2, 8, 4, p, 16, 8, p, 16, 8, p, None, None, None, 1, 0, None, p, p, None, p + 4, 1 << 30, None) == ARG
+    assert L.asr_rms_norm_bwd(0, p, 8, p, 8, None, 0, p, p, None, 0, 3, 8, p, p, p + 4, 1 << 30, None) == ARG
 
 
 def test_plain_forms_against_differences():
