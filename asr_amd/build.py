@@ -19,6 +19,10 @@ _NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 FILE_FLAGS = {'gemm.hip': ['-fno-slp-vectorize']}
 FILE_FLAGS.update({f: _NO_PACKED_FP32 for f in ('conv.hip', 'sscan_fwd.hip', 'sscan_bwd.hip', 'rmsnorm.hip',
                                                 'gradclip.hip')})
+# sscan_bwd.hip: with more than 16 states a lane's adjoints and rates of all groups of states are indexed arrays that belong in
+# scratch; promoted to registers they push a tile's states out (64 states: 210 spilled registers, T 512, B 16, D 2048, bf16 1314 us
+# instead of 1145).
+FILE_FLAGS['sscan_bwd.hip'] = _NO_PACKED_FP32 + ['-mllvm', '-disable-promote-alloca-to-vector=1']
 
 
 def file_flags(src):

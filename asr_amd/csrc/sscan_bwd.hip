@@ -37,16 +37,18 @@ __device__ __forceinline__ float sum16(const float (&v)[16], int lane) {
 
 // PRE: the adjoint a chunk hands to the one in front of it when nothing comes in from behind, and its sum of delta.
 // Behind a tile's first adjoints, when the first of its states have left their registers, the tile in front of it is called from
-// memory; it goes into the other half of the input buffers behind the tile's first barrier, beside the joins.  (Called a tile
+// memory; it goes into the input buffers behind the tile's first barrier, beside the joins.  (Called a tile
 // earlier, as the forward pass does, it costs 30 registers where they are scarcest: one wave per SIMD less, or spills; called
 // half way through the adjoints the spills are 28 registers, and T 2048, B 16, D 2048, bf16 takes 937 us instead of 886.)
 template <typename TY, int SPL, int NB, bool PRE>
-__global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanArgs p) {
+__global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
     constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RS = 8 / SPL;    // RS frames give sixteen sums
     constexpr int RB = (TS * NP + 255) / 256;
-    __shared__ float2 s_du[2][TS][64];
-    __shared__ float s_dy[2][TS][64];
-    __shared__ __attribute__((aligned(16))) float s_B[2][PRE ? 1 : TS * NP], s_C[2][TS * NP];
+    // the main pass places a tile's inputs when all waves are through with the last one's: one buffer; PRE before that: two
+    constexpr int HALVES = PRE ? 2 : 1;
+    __shared__ float2 s_du[HALVES][TS][64];
+    __shared__ float s_dy[HALVES][TS][64];
+    __shared__ __attribute__((aligned(16))) float s_B[HALVES][PRE ? 1 : TS * NP], s_C[HALVES][TS * NP];
     __shared__ float2 s_s[PRE ? 1 : 4][PRE ? 1 : TS][64];
     __shared__ float s_y[PRE ? 1 : 4][PRE ? 1 : TS][64];
     __shared__ float s_bc[PRE ? 1 : TS * 2 * NP];
@@ -140,12 +142,12 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
     // a tile; FULL: it and the one in front of it hold valid frames alone, and all lanes have a channel
     const auto walk = [&](int tile, auto full) {
         constexpr bool FULL = decltype(full)::value;
-        const int half = (q.t1 - 1 - tile) & 1, sb = tile * TS;
+        const int half = PRE ? (q.t1 - 1 - tile) & 1 : 0, sb = tile * TS;
 #pragma unroll
         for (int i = 0; i < 4; ++i) { rx[i] = nx[i]; rs[i] = ns[i]; rg[i] = ng[i]; }
         if (PRE) {
             if (FULL || tile > q.t0) fetch(tile - 1, full);
-#pragma unroll
+#pragma unroll(NB == 1 ? TS : 4)
             for (int t = TS - 1; t >= 0; --t) {
                 const float de = s_du[half][t][lane].x, dy = s_dy[half][t][lane];
 #pragma unroll
@@ -157,7 +159,8 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
                 if (w == 0) dsum += de;
             }
         } else {
-#pragma unroll
+            // one group of states at a time: of two, the registers hold neither (r, A2 and dA of several groups lie in scratch)
+#pragma unroll 1
             for (int m = 0; m < NB; ++m) {
                 float a[TS][SPL], h[TS][SPL], h0[SPL], da[SPL];    // da: a tile's part of dA: no sum runs over all frames
                 if (m == 0) {
@@ -226,19 +229,22 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void sstate_bwd_kernel(SscanA
             return;
         }
         __syncthreads();
-        if (FULL || tile > q.t0) place(tile - 1, half ^ 1, full);      // beside the joins below
+        // the next inputs go in beside the joins below: a thread has read its own frames' delta and dy before it replaces them
+        float de[4], dy[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { de[i] = s_du[half][w * 4 + i][lane].x; dy[i] = s_dy[half][w * 4 + i][lane]; }
+        if (FULL || tile > q.t0) place(tile - 1, 0, full);
         const int s0 = sb + w * 4;
         float ox[4], odt[4], oz[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int t = w * 4 + i;
-            const float de = s_du[half][t][lane].x, dy = s_dy[half][t][lane];
             const float2 a = s_s[0][t][lane], b = s_s[1][t][lane], c = s_s[2][t][lane], e = s_s[3][t][lane];
             const float s1 = (a.x + b.x) + (c.x + e.x), s2 = (a.y + b.y) + (c.y + e.y);
-            ox[i] = __builtin_fmaf(de, s1, Dk * dy);
+            ox[i] = __builtin_fmaf(de[i], s1, Dk * dy[i]);
             odt[i] = __builtin_fmaf(rx[i], s1, s2 * LN2) * rs[i];
             oz[i] = rg[i] * (((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i]);
-            accD = __builtin_fmaf(dy, rx[i], accD);     // frames of the padding give zeros
+            accD = __builtin_fmaf(dy[i], rx[i], accD);     // frames of the padding give zeros
             accb += odt[i];
         }
         const KArgs k = kargs();
