@@ -27,8 +27,9 @@ def _fail(msg):
     raise ValueError(msg)
 
 
-# the handle alone: torch.cuda.current_stream() makes an object of it
+# the handle and the index alone: torch.cuda.current_stream() makes an object, torch.cuda.current_device() looks for a first use
 _stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
 
 
 def _p(t):
@@ -68,6 +69,10 @@ def _par(name, t, shape, dev, like=None):
     return t.data_ptr()
 
 
+def _vec(t, n, dev):
+    return t.shape == (n,) and t.dtype is torch.float32 and t.is_contiguous() and t.get_device() == dev
+
+
 def _type(name, t):
     k = _DTYPES.get(t.dtype)
     if k is None:
@@ -83,7 +88,7 @@ def _gpu(dev):
 
 def _call(what, dev, fn, *args):
     """fn(*args, the current stream of device dev), with that device current"""
-    if torch.cuda.current_device() == dev:
+    if _current() == dev:
         rc = fn(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -138,7 +143,7 @@ def causal_conv_fwd(x, w, bias=None, state=None, lens=None, act='silu', reverse=
     kind, T, B, D, K, dev, st, pw, pb, ps, pl, silu = _conv_args(x, w, bias, state, lens, act)
     _gpu(dev)
     out = _new(x)
-    new = torch.empty((K - 1, B, D), dtype=x.dtype, device=x.device) if want_state else None
+    new = torch.empty(K - 1, B, D, dtype=x.dtype, device=x.device) if want_state else None
     _call('asr_conv_fwd', dev, _lib.lib().asr_conv_fwd, kind, T, B, D, K, x.data_ptr(), st[0], st[1], pw, pb, ps, pl, silu,
           int(reverse), out.data_ptr(), B * D, D, _p(new))
     return out, new
@@ -154,7 +159,7 @@ def causal_conv_bwd(dout, x, w, bias=None, state=None, lens=None, act='silu', re
     L = _lib.lib()
     dx = _new(x)
     dwb = torch.empty(D * (K + 1), dtype=torch.float32, device=x.device)
-    ds = torch.empty((K - 1, B, D), dtype=x.dtype, device=x.device) if state is not None else None
+    ds = _new(state)
     need = L.asr_conv_bwd_ws_bytes(T, B, D, K)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _call('asr_conv_bwd', dev, L.asr_conv_bwd, kind, T, B, D, K, dout.data_ptr(), so[0], so[1], x.data_ptr(), st[0], st[1], pw,
@@ -165,24 +170,37 @@ def causal_conv_bwd(dout, x, w, bias=None, state=None, lens=None, act='silu', re
 def causal_conv_step(x, state, w, bias=None, act='silu'):
     """One frame: x (B, D), state (K-1, B, D), which moves on in place.  -> out (B, D).  Equal to causal_conv_fwd over one
     frame."""
+    sh, ty, dev, sx, sw = x.shape, x.dtype, x.get_device(), x.stride(), w.shape
+    kind = _DTYPES.get(ty)
+    # everything in one expression, and name by name where that fails, as in selective_scan_step
+    if kind is None or dev < 0 or len(sh) != 2 or len(sw) != 2 or (act != 'silu' and act is not None) or not (
+            sw[0] == sh[1] > 0 and 2 <= sw[1] <= MAX_TAPS and state.shape == (sw[1] - 1, sh[0], sh[1]) and state.dtype is ty
+            and w.dtype is torch.float32 and sx[1] == 1 and state.is_contiguous() and w.is_contiguous()
+            and dev == state.get_device() == w.get_device() and (bias is None or _vec(bias, sh[1], dev))):
+        _conv_step_refusal(x, state, w, bias, act)
+    out = _new(x)
+    _call('asr_conv_step', dev, _lib.lib().asr_conv_step, kind, sh[0], sh[1], sw[1], x.data_ptr(), sx[0], state.data_ptr(),
+          w.data_ptr(), _p(bias), 1 if act else 0, out.data_ptr(), sh[1])
+    return out
+
+
+def _conv_step_refusal(x, state, w, bias, act):
+    """says what is wrong with a single frame's arguments (and accepts axes of one value with any stride)"""
     if x.dim() != 2:
         _fail('x: expected (B, D), got %d axes' % x.dim())
-    sh = x.shape
-    B, D = sh
+    B, D = x.shape
     K = _taps(w)
-    ty, dev = x.dtype, x.get_device()
-    kind = _type('x', x)
+    _type('x', x)
     if D < 1:
         _fail('x: no channels')
-    st = _act('x', x, sh, ty, dev)
-    pw = _par('w', w, (D, K), dev)
-    pb = _par('bias', bias, (D,), dev) if bias is not None else None
-    ps = _par('state', state, (K - 1, B, D), dev, ty)
-    silu = _act_kind(act)
+    ty, dev = x.dtype, x.get_device()
+    _act('x', x, (B, D), ty, dev)
+    _par('w', w, (D, K), dev)
+    if bias is not None:
+        _par('bias', bias, (D,), dev)
+    _par('state', state, (K - 1, B, D), dev, ty)
+    _act_kind(act)
     _gpu(dev)
-    out = _new(x)
-    _call('asr_conv_step', dev, _lib.lib().asr_conv_step, kind, B, D, K, x.data_ptr(), st[0], ps, pw, pb, silu, out.data_ptr(), D)
-    return out
 
 
 # ---------------------------------------------------------------------------------------------- selective scan
@@ -232,7 +250,7 @@ def selective_scan_fwd(x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, h0=None, 
     L = _lib.lib()
     f32, on = torch.float32, x.device
     out = _new(x)
-    h = torch.empty((B, Dn, N), dtype=f32, device=on)
+    h = torch.empty(B, Dn, N, dtype=f32, device=on)
     saved = torch.empty(L.asr_sscan_ckpt_floats(T, B, Dn, N), dtype=f32, device=on) if train else None
     need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 0)
     ws = torch.empty(need, dtype=torch.uint8, device=on) if need else None
@@ -268,25 +286,43 @@ def selective_scan_bwd(dout, x, dt, A, Bm, Cm, saved, D=None, z=None, dt_bias=No
 
 def selective_scan_step(h, x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, softplus=True):
     """One frame of selective_scan_fwd: h (B, D, N) moves on in place; x, dt, z (B, D); Bm, Cm (B, G, N).  -> out (B, D)."""
+    sh, ty, dev = x.shape, x.dtype, x.get_device()
+    kind = _DTYPES.get(ty)
+    sx, sd, sB, sC = x.stride(), dt.stride(), Bm.stride(), Cm.stride()
+    sz = z.stride() if z is not None else sx
+    sb, sA = Bm.shape, A.shape
+    # a stream's frame is a few microseconds of work: everything is looked at in one expression, and name by name where that fails
+    if kind is None or dev < 0 or len(sh) != 2 or len(sb) != 3 or len(sA) != 2 or not (
+            sh[1] > 0 and sb[1] > 0 and sh[1] % sb[1] == 0 and dt.shape == sh and Cm.shape == sb and sb[0] == sh[0]
+            and sA[0] == sh[1] and sA[1] == sb[2] and 1 <= sA[1] <= MAX_STATES and h.shape == (sh[0], sh[1], sA[1])
+            and dt.dtype is ty and Bm.dtype is ty and Cm.dtype is ty and A.dtype is h.dtype is torch.float32
+            and sx[1] == sd[1] == sz[1] == sB[2] == sC[2] == 1 and A.is_contiguous() and h.is_contiguous()
+            and dev == dt.get_device() == Bm.get_device() == Cm.get_device() == A.get_device() == h.get_device()
+            and (z is None or (z.shape == sh and z.dtype is ty and z.get_device() == dev))
+            and (D is None or _vec(D, sh[1], dev)) and (dt_bias is None or _vec(dt_bias, sh[1], dev))):
+        _step_refusal(h, x, dt, A, Bm, Cm, D, z, dt_bias)
+    out = _new(x)
+    _call('asr_sscan_step', dev, _lib.lib().asr_sscan_step, kind, sh[0], sh[1], sA[1], sb[1], h.data_ptr(), x.data_ptr(), sx[0],
+          dt.data_ptr(), sd[0], A.data_ptr(), Bm.data_ptr(), sB[0], sB[1], Cm.data_ptr(), sC[0], sC[1], _p(D), _p(z), sz[0],
+          _p(dt_bias), 1 if softplus else 0, out.data_ptr(), sh[1])
+    return out
+
+
+def _step_refusal(h, x, dt, A, Bm, Cm, D, z, dt_bias):
+    """says what is wrong with a single frame's arguments (and accepts axes of one value with any stride)"""
     if x.dim() != 2:
         _fail('x: expected (B, D), got %d axes' % x.dim())
     sh = B, Dn = x.shape
     N, G = _states(A, Bm, Dn, 3)
-    kind, ty, dev = _type('x', x), x.dtype, x.get_device()
-    sx = _act('x', x, sh, ty, dev)
-    sd = _act('dt', dt, sh, ty, dev)
-    pA = _par('A', A, (Dn, N), dev)
-    sB = _act('Bm', Bm, (B, G, N), ty, dev)
-    sC = _act('Cm', Cm, (B, G, N), ty, dev)
-    pz, sz = (z.data_ptr(), _act('z', z, sh, ty, dev)[0]) if z is not None else (None, 0)
-    pD = _par('D', D, (Dn,), dev) if D is not None else None
-    pb = _par('dt_bias', dt_bias, (Dn,), dev) if dt_bias is not None else None
-    ph = _par('h', h, (B, Dn, N), dev)
+    _type('x', x)
+    ty, dev = x.dtype, x.get_device()
+    for name, t, shape in (('x', x, sh), ('dt', dt, sh), ('Bm', Bm, (B, G, N)), ('Cm', Cm, (B, G, N)), ('z', z, sh)):
+        if t is not None:
+            _act(name, t, shape, ty, dev)
+    for name, t, shape in (('A', A, (Dn, N)), ('D', D, (Dn,)), ('dt_bias', dt_bias, (Dn,)), ('h', h, (B, Dn, N))):
+        if t is not None:
+            _par(name, t, shape, dev)
     _gpu(dev)
-    out = _new(x)
-    _call('asr_sscan_step', dev, _lib.lib().asr_sscan_step, kind, B, Dn, N, G, ph, x.data_ptr(), sx[0], dt.data_ptr(), sd[0], pA,
-          Bm.data_ptr(), sB[0], sB[1], Cm.data_ptr(), sC[0], sC[1], pD, pz, sz, pb, 1 if softplus else 0, out.data_ptr(), Dn)
-    return out
 
 
 # ---------------------------------------------------------------------------------------------- norm
@@ -311,7 +347,7 @@ def add_rms_norm_fwd(x, w, residual=None, eps=1e-6):
     _gpu(dev)
     y = _new(x)
     r = _new(residual)
-    rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
     _call('asr_rms_norm_fwd', dev, _lib.lib().asr_rms_norm_fwd, kind, x.data_ptr(), sx[0], pr, sr, pw, rows, n, eps,
           y.data_ptr(), _p(r), rstd.data_ptr())
     return y, (x if r is None else r), rstd
@@ -371,7 +407,7 @@ def clip_list(tensors, max_norm, eps=1e-7):
     L = _lib.lib()
     csizes = (C.c_longlong * n)(*sizes)
     need = L.asr_clip_list_ws_bytes(n, csizes)
-    norm = torch.empty((1,), dtype=torch.float32, device=on)
+    norm = torch.empty(1, dtype=torch.float32, device=on)
     ws = torch.empty(need, dtype=torch.uint8, device=on)
     _call('asr_clip_list', dev, L.asr_clip_list, n, (C.c_int * n)(*kinds), (C.c_void_p * n)(*[t.data_ptr() for t in src]),
           (C.c_void_p * n)(*dst), csizes, max_norm, eps, norm.data_ptr(), ws.data_ptr(), need)

@@ -52,7 +52,8 @@ def test_conv_step_and_gradient_refusals():
     x, st, w = torch.zeros(2, 8), torch.zeros(3, 2, 8), torch.zeros(8, 4)
     for args, msg in [((torch.zeros(1, 2, 8), st, w), 'axes'), ((x, torch.zeros(2, 2, 8), w), 'shape'), ((x, st.half(), w), 'like'),
                       ((x, torch.zeros(3, 8, 2).transpose(1, 2), w), 'stride'), ((x, torch.zeros(2, 3, 8).transpose(0, 1), w), 'contiguous'),
-                      ((x, st, torch.zeros(8, 9)), 'K <= 8'), ((x, st, w), 'GPU')]:
+                      ((x, st, torch.zeros(8, 9)), 'K <= 8'), ((x[:, :0], st[..., :0], w[:0]), 'channels'), ((x.double(), st, w), 'float64'),
+                      ((x, st, w[:4]), 'shape'), ((x, st, w, torch.zeros(7)), 'bias'), ((x, st, w, None, 'relu'), 'silu'), ((x, st, w), 'GPU')]:
         with pytest.raises(ValueError, match=msg):
             ops.causal_conv_step(*args)
     with pytest.raises(ValueError, match='dout'):
@@ -99,7 +100,12 @@ def test_scan_gradient_and_step_refusals():
     for args, kw, msg in [((h, torch.zeros(1, 2, 8), x, A, b, b), {}, 'axes'), ((h.half(), x, x, A, b, b), {}, 'float32'),
                           ((h[:1], x, x, A, b, b), {}, 'h:'), ((h, x, x, A, torch.zeros(2, 3, 4), b), {}, 'divide'), ((h, x, x, A, b, b[:, :1]), {}, 'Cm'),
                           ((h, x, x, A, b, b), dict(z=x.half()), 'like'), ((h, x, x, A, b, b), {}, 'GPU'),
-                          ((torch.zeros(2, 4, 8).transpose(1, 2), x, x, A, b, b), {}, 'contiguous')]:
+                          ((torch.zeros(2, 4, 8).transpose(1, 2), x, x, A, b, b), {}, 'contiguous'),
+                          ((h, x, x, A, b[:, :0], b[:, :0]), {}, 'divide'), ((h[:, :0], x[:, :0], x[:, :0], A[:0], b, b), {}, 'divide'),
+                          ((h, x.double(), x, A, b, b), {}, 'float64'), ((h, x, x[:1], A, b, b), {}, 'dt'), ((h, x, x, A[:4], b, b), {}, 'A:'),
+                          ((h, x, x, A, b, b), dict(D=x[0, :4]), 'D:'), ((h, x, x, A, b, b), dict(dt_bias=x[0].half()), 'dt_bias'),
+                          ((h, torch.zeros(2, 16)[:, ::2], x, A, b, b), {}, 'stride 1'), ((h, x, x, torch.zeros(8, 65), b, b), {}, 'N <= 64'),
+                          ((h, x, x, A, b[0], b), {}, 'axes')]:
         with pytest.raises(ValueError, match=msg):
             ops.selective_scan_step(*args, **kw)
 
