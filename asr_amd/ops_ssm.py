@@ -12,6 +12,7 @@ torch, so calls on several streams and calls captured into graphs share nothing.
 A wrong argument raises ValueError before anything is launched.
 """
 import ctypes as C
+import struct
 
 import torch
 
@@ -216,25 +217,61 @@ def _states(A, Bm, Dn, axes):
     return A.shape[1], G
 
 
+# the descriptor's members in their order: eight ints, then pointers (0 for NULL) and strides
+_MEMBERS = struct.Struct('8i%dq' % (len(_lib.SscanDesc._fields_) - 8))
+
+
+def _desc(*members):
+    return C.byref(_lib.SscanDesc.from_buffer_copy(_MEMBERS.pack(*members)))
+
+
+_FORWARD_ONLY = (0,) * (len(_lib.SscanDesc._fields_) - 35)      # the members behind ckpt
+
+
+def _a(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, lens, softplus, reverse):
     """the sizes, the device, and the descriptor's members up to h0"""
+    sh, ty, dev = x.shape, x.dtype, x.get_device()
+    kind = _DTYPES.get(ty)
+    sx, sd, sB, sC = x.stride(), dt.stride(), Bm.stride(), Cm.stride()
+    sz = z.stride() if z is not None else sx
+    sb, sA = Bm.shape, A.shape
+    if kind is None or len(sh) != 3 or len(sb) != 4 or len(sA) != 2 or not (
+            sh[2] > 0 and sb[2] > 0 and sh[2] % sb[2] == 0 and dt.shape == sh and Cm.shape == sb and sb[:2] == sh[:2]
+            and (z is None or (z.shape == sh and z.dtype is ty and z.get_device() == dev))
+            and sA[0] == sh[2] and sA[1] == sb[3] and 1 <= sA[1] <= MAX_STATES
+            and dt.dtype is ty and Bm.dtype is ty and Cm.dtype is ty and A.dtype is torch.float32
+            and sx[2] == sd[2] == sz[2] == sB[3] == sC[3] == 1 and A.is_contiguous()
+            and dev == dt.get_device() == Bm.get_device() == Cm.get_device() == A.get_device()
+            and (D is None or _vec(D, sh[2], dev)) and (dt_bias is None or _vec(dt_bias, sh[2], dev))):
+        _scan_refusal(x, dt, A, Bm, Cm, D, z, dt_bias)
+    T, B, Dn = sh
+    N, G = sA[1], sb[2]
+    if h0 is not None:
+        _par('h0', h0, (B, Dn, N), dev)
+    return (T, B, Dn, N, G), dev, (T, B, Dn, N, G, kind, 1 if reverse else 0, 1 if softplus else 0, _lens(lens, B, dev) or 0,
+                                   x.data_ptr(), sx[0], sx[1], dt.data_ptr(), sd[0], sd[1], _a(z), sz[0], sz[1], Bm.data_ptr(),
+                                   sB[0], sB[1], sB[2], Cm.data_ptr(), sC[0], sC[1], sC[2], A.data_ptr(), _a(D), _a(dt_bias),
+                                   _a(h0))
+
+
+def _scan_refusal(x, dt, A, Bm, Cm, D, z, dt_bias):
+    """says what is wrong with a sequence's arguments (and accepts axes of one value with any stride)"""
     if x.dim() != 3:
         _fail('x: expected (T, B, D), got %d axes' % x.dim())
     sh = T, B, Dn = x.shape
     N, G = _states(A, Bm, Dn, 4)
-    kind, ty, dev = _type('x', x), x.dtype, x.get_device()
-    sx = _act('x', x, sh, ty, dev)
-    sd = _act('dt', dt, sh, ty, dev)
-    pA = _par('A', A, (Dn, N), dev)
-    sB = _act('Bm', Bm, (T, B, G, N), ty, dev)
-    sC = _act('Cm', Cm, (T, B, G, N), ty, dev)
-    pz, sz = (z.data_ptr(), _act('z', z, sh, ty, dev)) if z is not None else (None, (0, 0))
-    pD = _par('D', D, (Dn,), dev) if D is not None else None
-    pb = _par('dt_bias', dt_bias, (Dn,), dev) if dt_bias is not None else None
-    ph = _par('h0', h0, (B, Dn, N), dev) if h0 is not None else None
-    return (T, B, Dn, N, G), dev, (T, B, Dn, N, G, kind, int(reverse), int(softplus), _lens(lens, B, dev), x.data_ptr(), sx[0],
-                                   sx[1], dt.data_ptr(), sd[0], sd[1], pz, sz[0], sz[1], Bm.data_ptr(), sB[0], sB[1], sB[2],
-                                   Cm.data_ptr(), sC[0], sC[1], sC[2], pA, pD, pb, ph)
+    _type('x', x)
+    ty, dev = x.dtype, x.get_device()
+    for name, t, shape in (('x', x, sh), ('dt', dt, sh), ('Bm', Bm, (T, B, G, N)), ('Cm', Cm, (T, B, G, N)), ('z', z, sh)):
+        if t is not None:
+            _act(name, t, shape, ty, dev)
+    for name, t, shape in (('A', A, (Dn, N)), ('D', D, (Dn,)), ('dt_bias', dt_bias, (Dn,))):
+        if t is not None:
+            _par(name, t, shape, dev)
 
 
 def selective_scan_fwd(x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, h0=None, lens=None, softplus=True, reverse=False,
@@ -254,8 +291,8 @@ def selective_scan_fwd(x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, h0=None, 
     saved = torch.empty(L.asr_sscan_ckpt_floats(T, B, Dn, N), dtype=f32, device=on) if train else None
     need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 0)
     ws = torch.empty(need, dtype=torch.uint8, device=on) if need else None
-    desc = _lib.SscanDesc(*members, out.data_ptr(), B * Dn, Dn, h.data_ptr(), _p(saved))
-    _call('asr_sscan_fwd', dev, L.asr_sscan_fwd, C.byref(desc), _p(ws), need)
+    desc = _desc(*members, out.data_ptr(), B * Dn, Dn, h.data_ptr(), _a(saved), *_FORWARD_ONLY)
+    _call('asr_sscan_fwd', dev, L.asr_sscan_fwd, desc, _p(ws), need)
     return out, h, saved
 
 
@@ -270,17 +307,16 @@ def selective_scan_bwd(dout, x, dt, A, Bm, Cm, saved, D=None, z=None, dt_bias=No
     if saved is None or saved.shape != (L.asr_sscan_ckpt_floats(T, B, Dn, N),):
         _fail('saved: not what selective_scan_fwd(..., train=True) returned for these shapes')
     ps = _par('saved', saved, saved.shape, dev)
-    ph = _par('dh_last', dh_last, (B, Dn, N), dev) if dh_last is not None else None
+    ph = _par('dh_last', dh_last, (B, Dn, N), dev) if dh_last is not None else 0
     _gpu(dev)
     on = x.device
     g = {'x': _new(x), 'dt': _new(dt), 'A': _new(A), 'B': _new(Bm), 'C': _new(Cm), 'D': _new(D), 'z': _new(z),
          'dt_bias': _new(dt_bias), 'h0': _new(h0)}
     need = L.asr_sscan_ws_bytes(T, B, Dn, N, G, 1)
     ws = torch.empty(need, dtype=torch.uint8, device=on)
-    desc = _lib.SscanDesc(*members, None, 0, 0, None, ps, dout.data_ptr(), so[0], so[1], ph, g['x'].data_ptr(),
-                          g['dt'].data_ptr(), _p(g['z']), g['B'].data_ptr(), g['C'].data_ptr(), g['A'].data_ptr(),
-                          _p(g['D']), _p(g['dt_bias']), _p(g['h0']))
-    _call('asr_sscan_bwd', dev, L.asr_sscan_bwd, C.byref(desc), ws.data_ptr(), need)
+    desc = _desc(*members, 0, 0, 0, 0, ps, dout.data_ptr(), so[0], so[1], ph, g['x'].data_ptr(), g['dt'].data_ptr(), _a(g['z']),
+                 g['B'].data_ptr(), g['C'].data_ptr(), g['A'].data_ptr(), _a(g['D']), _a(g['dt_bias']), _a(g['h0']))
+    _call('asr_sscan_bwd', dev, L.asr_sscan_bwd, desc, ws.data_ptr(), need)
     return g
 
 
@@ -294,11 +330,11 @@ def selective_scan_step(h, x, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, softp
     # a stream's frame is a few microseconds of work: everything is looked at in one expression, and name by name where that fails
     if kind is None or dev < 0 or len(sh) != 2 or len(sb) != 3 or len(sA) != 2 or not (
             sh[1] > 0 and sb[1] > 0 and sh[1] % sb[1] == 0 and dt.shape == sh and Cm.shape == sb and sb[0] == sh[0]
+            and (z is None or (z.shape == sh and z.dtype is ty and z.get_device() == dev))
             and sA[0] == sh[1] and sA[1] == sb[2] and 1 <= sA[1] <= MAX_STATES and h.shape == (sh[0], sh[1], sA[1])
             and dt.dtype is ty and Bm.dtype is ty and Cm.dtype is ty and A.dtype is h.dtype is torch.float32
             and sx[1] == sd[1] == sz[1] == sB[2] == sC[2] == 1 and A.is_contiguous() and h.is_contiguous()
             and dev == dt.get_device() == Bm.get_device() == Cm.get_device() == A.get_device() == h.get_device()
-            and (z is None or (z.shape == sh and z.dtype is ty and z.get_device() == dev))
             and (D is None or _vec(D, sh[1], dev)) and (dt_bias is None or _vec(dt_bias, sh[1], dev))):
         _step_refusal(h, x, dt, A, Bm, Cm, D, z, dt_bias)
     out = _new(x)

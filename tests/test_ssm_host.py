@@ -23,6 +23,12 @@ def test_descriptor_layout_matches_ctypes(tmp_path):
     subprocess.check_call(['gcc', '-std=c99', '-Wall', '-Werror', '-I', os.path.join(ROOT, 'include'), str(prog), '-o', str(exe)])
     got = [int(v) for v in subprocess.check_output([str(exe)]).decode().split()]
     assert got == [getattr(_lib.SscanDesc, n).offset for n in names] + [C.sizeof(_lib.SscanDesc)]
+    # the wrapper packs the members as eight ints and 8-byte words
+    from asr_amd import ops_ssm
+    words = list(range(1, len(names) + 1))
+    d = _lib.SscanDesc.from_buffer_copy(ops_ssm._MEMBERS.pack(*words))
+    assert [getattr(d, n) for n in names] == words and ops_ssm._MEMBERS.size == C.sizeof(_lib.SscanDesc)
+    assert names.index('ckpt') + 1 + len(ops_ssm._FORWARD_ONLY) == len(names)
 
 
 def conv_args(**kw):
@@ -75,7 +81,8 @@ SCAN_BAD = [
     (dict(dt=torch.zeros(5, 2, 8).bfloat16()), 'like'), (dict(A=torch.zeros(8, 65)), 'N <= 64'), (dict(A=torch.zeros(8, 0)), 'N <= 64'),
     (dict(A=torch.zeros(8, 4).half()), 'float32'), (dict(A=torch.zeros(4, 8).t()), 'contiguous'), (dict(Bm=torch.zeros(5, 2, 4)), 'axes'),
     (dict(Bm=torch.zeros(5, 2, 3, 4)), 'divide'), (dict(Cm=torch.zeros(5, 2, 1, 4)), 'Cm'), (dict(Cm=torch.zeros(5, 2, 2, 8)[..., ::2]), 'stride 1'),
-    (dict(D=torch.zeros(4)), 'D'), (dict(z=torch.zeros(5, 2, 4)), 'z'), (dict(dt_bias=torch.zeros(8).half()), 'float32'),
+    (dict(D=torch.zeros(4)), 'D'), (dict(z=torch.zeros(5, 2, 4)), 'z'), (dict(z=torch.zeros(5, 2)), 'z'), (dict(dt=torch.zeros(5)), 'dt'),
+    (dict(x=torch.zeros(5, 2, 0), dt=torch.zeros(5, 2, 0), A=torch.zeros(0, 4)), 'divide'), (dict(Bm=torch.zeros(5, 2, 0, 4)), 'divide'), (dict(dt_bias=torch.zeros(8).half()), 'float32'),
     (dict(h0=torch.zeros(2, 4, 8)), 'h0'), (dict(lens=torch.zeros(2)), 'int32'), (dict(), 'GPU')]
 
 
@@ -105,7 +112,7 @@ def test_scan_gradient_and_step_refusals():
                           ((h, x.double(), x, A, b, b), {}, 'float64'), ((h, x, x[:1], A, b, b), {}, 'dt'), ((h, x, x, A[:4], b, b), {}, 'A:'),
                           ((h, x, x, A, b, b), dict(D=x[0, :4]), 'D:'), ((h, x, x, A, b, b), dict(dt_bias=x[0].half()), 'dt_bias'),
                           ((h, torch.zeros(2, 16)[:, ::2], x, A, b, b), {}, 'stride 1'), ((h, x, x, torch.zeros(8, 65), b, b), {}, 'N <= 64'),
-                          ((h, x, x, A, b[0], b), {}, 'axes')]:
+                          ((h, x, x, A, b[0], b), {}, 'axes'), ((h, x, x, A, b, b), dict(z=x[0]), 'z:')]:
         with pytest.raises(ValueError, match=msg):
             ops.selective_scan_step(*args, **kw)
 
