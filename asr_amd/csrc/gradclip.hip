@@ -83,7 +83,7 @@ __global__ __launch_bounds__(1024) void clip_norm_kernel(const double* __restric
     }
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __device__ __forceinline__ void chunk_scale(const T* p, T* q, int n, float m) {
     constexpr int V = 16 / sizeof(T);
     const int nv = n / V;
@@ -91,19 +91,26 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* q, int n, float m) {
         typename Any16<T>::type v = *(const typename Any16<T>::type*)(p + i * V);
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = (T)((float)v[e] * m);
-        *(typename Any16<T>::type*)(q + i * V) = v;
+        if constexpr (STREAM) __builtin_nontemporal_store(v, (typename Any16<T>::type*)(q + i * V));
+        else *(typename Any16<T>::type*)(q + i * V) = v;
     }
     for (int i = nv * V + threadIdx.x; i < n; i += 256) stf(q + i, ldf(p + i) * m);
 }
 
+// STREAM: results that do not stay in the caches.  From 64 MiB on they would push out the inputs that this second pass still has
+// to read: with a momentum step behind it that reads the results, 64 / 128 / 256 / 512 MiB of f32 take 122 / 299 / 662 / 1323 us
+// instead of 141 / 309 / 678 / 1331; at 32 MiB the step misses them (80 us instead of 67), at 8 MiB there is no difference.
+#define STREAM_BYTES (64ll << 20)
+template <bool STREAM>
 __global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const float* __restrict__ mult) {
-    const int t = find_tensor(l, blockIdx.x);
-    const long long at = (long long)(blockIdx.x - l.first[t]) * CHUNK;
+    const int c = gridDim.x - 1 - blockIdx.x;          // what was read last, first: it is in the caches
+    const int t = find_tensor(l, c);
+    const long long at = (long long)(c - l.first[t]) * CHUNK;
     const int n = (int)min((long long)CHUNK, l.size[t] - at);
     const float m = mult[0];
-    if (l.dtype[t] == ASR_F32) chunk_scale((const float*)l.src[t] + at, (float*)l.dst[t] + at, n, m);
-    else if (l.dtype[t] == ASR_BF16) chunk_scale((const bf16_t*)l.src[t] + at, (bf16_t*)l.dst[t] + at, n, m);
-    else chunk_scale((const f16_t*)l.src[t] + at, (f16_t*)l.dst[t] + at, n, m);
+    if (l.dtype[t] == ASR_F32) chunk_scale<float, STREAM>((const float*)l.src[t] + at, (float*)l.dst[t] + at, n, m);
+    else if (l.dtype[t] == ASR_BF16) chunk_scale<bf16_t, STREAM>((const bf16_t*)l.src[t] + at, (bf16_t*)l.dst[t] + at, n, m);
+    else chunk_scale<f16_t, STREAM>((const f16_t*)l.src[t] + at, (f16_t*)l.dst[t] + at, n, m);
 }
 
 // ---------------------------------------------------------------- C entry
@@ -121,12 +128,13 @@ extern "C" int asr_clip_list(int count, const int* dtypes, const void* const* sr
                              size_t ws_bytes, hipStream_t stream) {
     if (count < 0 || !norm_out || !(max_norm >= 0.f) || !(eps >= 0.f)) return ASR_ERR_ARG;
     if (count && (!dtypes || !src || !dst || !sizes)) return ASR_ERR_ARG;
-    long long total = 0;
+    long long total = 0, bytes = 0;
     for (int i = 0; i < count; ++i) {
         if (dtypes[i] < ASR_F32 || dtypes[i] > ASR_F16 || sizes[i] < 0) return ASR_ERR_ARG;
         if (sizes[i] && (!src[i] || !dst[i])) return ASR_ERR_ARG;
         if (sizes[i] > (1ll << 40)) return ASR_ERR_LIMIT;
         total += chunks_of(sizes[i]);
+        bytes += sizes[i] * (long long)elem_size(dtypes[i]);
     }
     if (total >= (1 << 24)) return ASR_ERR_LIMIT;                // 2^32 work items a launch
     if (!ws || ws_bytes < asr_clip_list_ws_bytes(count, sizes)) return ASR_ERR_WS;
@@ -150,7 +158,9 @@ extern "C" int asr_clip_list(int count, const int* dtypes, const void* const* sr
             if (!l.count) break;
             l.first[l.count] = c;
             if (pass == 0) hipLaunchKernelGGL(clip_sq_kernel, dim3(c), dim3(256), 0, stream, l, at);
-            else hipLaunchKernelGGL(clip_scale_kernel, dim3(c), dim3(256), 0, stream, l, (const float*)mult);
+            else if (bytes >= STREAM_BYTES)
+                hipLaunchKernelGGL(clip_scale_kernel<true>, dim3(c), dim3(256), 0, stream, l, (const float*)mult);
+            else hipLaunchKernelGGL(clip_scale_kernel<false>, dim3(c), dim3(256), 0, stream, l, (const float*)mult);
             ASR_CHECK_LAUNCH();
             at += c;
         }
