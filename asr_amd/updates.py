@@ -77,13 +77,23 @@ class NormHandle(object):
     value = None
 
 
+class ScaledGrads(list, ClippedGrads):
+    """The scaled tensors of a list.  An updater that is given it, as the reference's scripts do, still finds how the network's
+    own gradients are to be clipped."""
+    def __init__(self, tensors, max_norm, epsilon):
+        list.__init__(self, tensors)
+        ClippedGrads.__init__(self, max_norm, epsilon)
+
+
 def total_norm_constraint(tensor_vars=None, max_norm=0.0, epsilon=1e-7, return_norm=False):
     """libs/lasagne_libs/updates.py:781-855 (lasagne.updates.total_norm_constraint).  A list of GPU tensors (gradients held
-    outside a network's flat buffer, such as those of asr_amd.ops.selective_scan_bwd) is clipped here and now: the scaled
-    tensors are returned, with the norm as a (1,) tensor if return_norm.  Anything else stands for the network's own
+    outside a network's flat buffer, such as those of asr_amd.ops.selective_scan_bwd) is clipped here and now: the list of the
+    scaled tensors is returned, with the norm as a (1,) tensor if return_norm.  Anything else stands for the network's own
     gradients, which the optimiser kernel scales when it reads them."""
-    if isinstance(tensor_vars, (list, tuple)) and tensor_vars and all(isinstance(t, torch.Tensor) for t in tensor_vars):
+    if isinstance(tensor_vars, (list, tuple)) and all(isinstance(t, torch.Tensor) for t in tensor_vars) and any(
+            t.is_cuda for t in tensor_vars):
         scaled, norm = ops.clip_list(tensor_vars, max_norm, epsilon)
+        scaled = ScaledGrads(scaled, max_norm, epsilon)
         return (scaled, norm) if return_norm else scaled
     cg = ClippedGrads(max_norm, epsilon)
     return (cg, NormHandle()) if return_norm else cg

@@ -4,6 +4,7 @@ import ctypes as C
 import os
 import subprocess
 
+import numpy as np
 import pytest
 import torch
 
@@ -133,11 +134,28 @@ def test_norm_and_list_refusals():
     for args, msg in [(([torch.zeros(3).long()], 1.0), 'int64'), (([torch.zeros(3)], -1.0), 'negative'), (([torch.zeros(3)], 1.0, -1.0), 'negative'),
                       (([torch.zeros(3)], 1.0), 'GPU')]:
         with pytest.raises(ValueError, match=msg):
-            updates.total_norm_constraint(*args)
+            ops.clip_list(*args)
     with pytest.raises(ValueError, match='none'):
         ops.clip_list([], 1.0)
     # a network's own gradients go on as before
-    assert isinstance(updates.total_norm_constraint(None, 1.0), updates.ClippedGrads)
+    for own in (None, [], [np.zeros(3)], [torch.zeros(3)]):
+        cg = updates.total_norm_constraint(own, 1.0)
+        assert type(cg) is updates.ClippedGrads and cg.max_norm == 1.0
+
+
+def test_updater_behind_a_clipped_list_still_clips(monkeypatch):
+    """adam(total_norm_constraint([tensors], 5)) clips the network's own gradients, as it does behind any other tensor_vars."""
+    from asr_amd import ops, updates
+
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+    ts = [torch.zeros(3).as_subclass(OnGpu), torch.zeros(2).as_subclass(OnGpu)]
+    monkeypatch.setattr(ops, 'clip_list', lambda tensors, max_norm, eps: ([t + 1 for t in tensors], torch.ones(1)))
+    scaled, norm = updates.total_norm_constraint(ts, 5.0, 1e-6, return_norm=True)
+    assert isinstance(scaled, list) and len(scaled) == 2 and float(norm) == 1.0
+    for updater in (updates.adam, updates.sgd):
+        step, _ = updater(scaled)
+        assert step.clip.max_norm == 5.0 and step.clip.epsilon == 1e-6
 
 
 def test_c_entries_refuse_before_they_launch():
