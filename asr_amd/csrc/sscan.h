@@ -68,6 +68,19 @@ __device__ __forceinline__ Place sscan_place(const SscanArgs& p) {
     return q;
 }
 
+// A log2(e), finite below: a padding frame's delta of zero must leave exp(delta A) at 1 whatever the rate is.
+__device__ __forceinline__ float rate2(float A) {
+    const float v = A * LOG2E;
+    return v < -3.0e38f ? -3.0e38f : v;
+}
+
+// h 2^k, a state carried over a whole chunk.  In three factors: of a state that grows (k > 0) 2^k may overflow where h 2^k does
+// not, or where h is zero and stays so.  (From k = 381 on any h but zero is infinite.)
+__device__ __forceinline__ float carried(float h, float k) {
+    const float e = __builtin_amdgcn_exp2f(fminf(k, 381.f) * (1.f / 3.f));
+    return h * e * e * e;
+}
+
 // A thread's share of a tile's rows: frames w*4 .. w*4+3 of its channel.  `base` is the row's own address (uniform), `off` the
 // channel's byte offset, so an access is a scalar address plus a 32-bit lane offset.  FULL: all frames are valid.  Otherwise
 // frames behind the row read its last one, and what they give is thrown away by the caller.

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
 #pragma unroll
         for (int j = 0; j < SPL; ++j) {
             const int n = (m * 4 + w) * SPL + j;
-            A2[m][j] = n < p.N ? p.A[(size_t)d * p.N + n] * LOG2E : 0.f;
+            A2[m][j] = n < p.N ? rate2(p.A[(size_t)d * p.N + n]) : 0.f;
             r[m][j] = (!PRE && p.dh_last && n < p.N) ? p.dh_last[((size_t)q.b * p.D + d) * p.N + n] : 0.f;
             dA[m][j] = 0.f;
         }
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
                 for (int i = 0; i < SPL; ++i) {
                     const int n = (m * 4 + w) * SPL + i;
                     const float rl = p.c_h[(((size_t)j * p.B + q.b) * NP + n) * p.D + d];
-                    r[m][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][i] * ds), r[m][i], rl);
+                    r[m][i] = carried(r[m][i], A2[m][i] * ds) + rl;
                 }
         }
     }

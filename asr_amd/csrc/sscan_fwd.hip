@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
 #pragma unroll
         for (int j = 0; j < SPL; ++j) {
             const int n = (m * 4 + w) * SPL + j;
-            A2[m][j] = n < p.N ? p.A[(size_t)d * p.N + n] * LOG2E : 0.f;
+            A2[m][j] = n < p.N ? rate2(p.A[(size_t)d * p.N + n]) : 0.f;
             h[m][j] = (!PRE && p.h0 && n < p.N) ? p.h0[((size_t)q.b * p.D + d) * p.N + n] : 0.f;
         }
     if (!PRE) {                       // the state this chunk starts from
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
                 for (int i = 0; i < SPL; ++i) {
                     const int n = (m * 4 + w) * SPL + i;
                     const float hl = p.c_h[(((size_t)j * p.B + q.b) * NP + n) * p.D + d];
-                    h[m][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[m][i] * ds), h[m][i], hl);
+                    h[m][i] = carried(h[m][i], A2[m][i] * ds) + hl;
                 }
         }
     }

@@ -287,6 +287,55 @@ def test_scan_extreme_steps():
     R.close(h, rh, 8 * T + 2 * N + 32, 'h')
 
 
+def test_scan_growing_states_over_chunks():
+    """Rates above zero over a time that is walked in chunks: a state that is still zero stays zero (a chunk's whole growth,
+    e^128 at 64 frames of delta = 2, is infinite in float32), and what enters near the end grows by e^2 a frame.  The roundings
+    of 20 growing frames are relative to what has grown: 8 a frame, as for a state that decays."""
+    from asr_amd import ops
+    T, B, D, N = 2048, 1, 64, 4
+    g = gen(11)
+    x = torch.zeros(T, B, D).cuda()
+    x[-20:] = rn(g, 20, B, D)
+    dt = torch.full((T, B, D), 2.0).cuda()
+    A = torch.tensor([1.0, 0.5, -0.5, -1.0]).repeat(D, 1).cuda()
+    Bm, Cm = rn(g, T, B, 1, N), rn(g, T, B, 1, N)
+    a = (x, dt, A, Bm, Cm)
+    out, h, saved = ops.selective_scan_fwd(*a, softplus=False, train=True)
+    ro, rh = R.scan(*[R.leaf(v, False) for v in a], softplus=False)
+    R.close(out, ro, 8 * 20 + 2 * N + 32, 'out')
+    R.close(h, rh, 8 * 20 + 2 * N + 32, 'h')
+    # the adjoint of the first 20 frames, with nothing behind them: dx = delta sum_n B dh
+    x.zero_()
+    out, h, saved = ops.selective_scan_fwd(*a, softplus=False, train=True)
+    assert not out.any() and not h.any()
+    do = torch.zeros(T, B, D).cuda()
+    do[:20] = rn(g, 20, B, D)
+    gr = ops.selective_scan_bwd(do, *a, saved, softplus=False)
+    lx = R.leaf(x)
+    ro, _ = R.scan(lx, *[R.leaf(v, False) for v in a[1:]], softplus=False)
+    ref, = torch.autograd.grad((ro * R.leaf(do, False)).sum(), lx)
+    R.close(gr['x'], ref, 4 * (8 * 20 + 2 * N + 32), 'dx')
+    for k in ('dt', 'A', 'C'):
+        assert not gr[k].any(), k                      # the state is zero all along
+
+
+def test_scan_infinite_decay():
+    """a rate of -inf (and one whose product with log2(e) overflows) forgets everything behind its own frame, exactly, in ragged
+    rows too; its state's share of dA is zero"""
+    from asr_amd import ops
+    T, B, D, N = 150, 3, 64, 8
+    lens = torch.tensor([150, 37, 0], dtype=torch.int32).cuda()
+    a, opt = scan_inputs(gen(21), T, B, D, N, 1, torch.float32)
+    a['A'][:, 0], a['A'][:, 1] = float('-inf'), -3e38
+    opt['h0'] = None
+    out, h, saved = ops.selective_scan_fwd(*a.values(), lens=lens, train=True, **opt)
+    ro, rh = R.scan(*[R.leaf(v, False) for v in a.values()], lens=lens.cpu(), **{k: R.leaf(v, False) for k, v in opt.items()})
+    R.close(out, ro, 8 * T + 2 * N + 32, 'out')
+    R.close(h, rh, 8 * T + 2 * N + 32, 'h')
+    gr = ops.selective_scan_bwd(rn(gen(2), T, B, D), *a.values(), saved, lens=lens, **opt)
+    assert all(v is None or torch.isfinite(v).all() for v in gr.values()) and not gr['A'][:, :2].any()
+
+
 def test_scan_shared_projections_by_expand():
     """B and C handed in with stride 0 over the rows: values shared, gradients per row"""
     from asr_amd import ops
