@@ -4,7 +4,8 @@
 // HBM-bound: a pass reads and writes every tensor once, a row stays in registers between its two uses.  r is rounded to the
 // activation type when it is stored; y is formed from the unrounded sum, and the backward pass forms that sum again from x and
 // the residual (one more read than the stored r would cost, but gradients of what was computed: with the stored r, dw is off by
-// the type's half step).
+// the type's half step).  Measured at 36192 rows x 1024, bf16, with a residual: forward 50 us (5.9 TB/s of the 0.30 GB of its four
+// tensors, some of them still in the Infinity Cache), backward 81 us (4.6 TB/s of 0.37 GB) and 5 for the parts of dw.
 #include "seq_common.h"
 
 // WPR waves share a row (1: four rows per workgroup, 4: one).  NV groups of V values per lane are held in registers.
@@ -203,8 +204,8 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const T* __restrict__
 // ---------------------------------------------------------------- C entries
 static bool al(const void* p, int b) { return ((uintptr_t)p & (b - 1)) == 0; }
 
-// How a row is held: V values at a time when the row's length, strides and addresses allow it, up to 32 values per lane; a
-// wave per row up to 64 * 16 values (no barrier), four waves above; wide = 0: the row does not fit the registers.
+// How a row is held: V values at a time when the row's length, strides and addresses allow it, up to 32 values per lane (16 single
+// ones); a wave per row up to 64 * 16 values (no barrier), four waves above; wide = 0: the row does not fit the registers.
 struct RmsPlan { int vec, nv, wpr, wide; };
 static RmsPlan rms_plan(int dtype, int n, bool vec) {
     const int V = vec ? 16 / (int)elem_size(dtype) : 1;
