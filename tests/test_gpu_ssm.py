@@ -358,7 +358,9 @@ def test_scan_shared_projections_by_expand():
 @pytest.mark.parametrize('rows,n,res,lay', [(1, 1, False, 'c'), (3, 64, True, 'c'), (5, 100, True, 'c'), (7, 512, True, 'half'),
                                             (9, 1000, True, 'odd'), (2, 1024, True, 'c'), (3, 1032, True, 'c'), (2, 2047, True, 'c'),
                                             (4, 4096, False, 'c'), (3, 8192, True, 'c'), (2, 5001, True, 'c'),
-                                            (2, 9000, True, 'c'), (2500, 40, True, 'c'), (2100, 1040, True, 'c'), (0, 16, True, 'c')])
+                                            (2, 9000, True, 'c'), (2500, 40, True, 'c'), (2100, 1040, True, 'c'), (0, 16, True, 'c'),
+                                            (6, 7, True, 'odd'), (6, 9, True, 'half'), (2100, 333, True, 'odd'), (1100, 1025, True, 'odd'),
+                                            (5, 8191, True, 'odd'), (5, 8193, True, 'odd'), (3, 20003, True, 'c')])
 def test_rms_norm(ty, rows, n, res, lay):
     from asr_amd import ops
     ty = TY[ty]
