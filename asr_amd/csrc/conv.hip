@@ -28,29 +28,32 @@ template <typename T, int V, int K>
 __device__ __forceinline__ void load_x(const ConvArgs& p, int s, int len, int b, int d, float* o) {
     if (s >= 0) {
         const int f = p.reverse ? len - 1 - s : s;
-        ldv<T, V>((const T*)p.x + f * p.x_st + b * p.x_sb + d, o);
+        ldu<T, V>((const T*)p.x + f * p.x_st + b * p.x_sb + d, o);
     } else if (p.state) {
-        ldv<T, V>((const T*)p.state + ((size_t)(s + K - 1) * p.B + b) * p.D + d, o);
+        ldu<T, V>((const T*)p.state + ((size_t)(s + K - 1) * p.B + b) * p.D + d, o);
     } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = 0.f;
     }
 }
 
-template <typename T, int V> using Raw = typename Vec<T, V>::type;
+template <typename T, int V> using Raw = typename AnyV<T, V>::type;
 template <typename T, int V> __device__ __forceinline__ float raw_at(const Raw<T, V>& r, int e) {
     if constexpr (V == 1) return (float)r; else return (float)r[e];
 }
 
+// Where D is no multiple of V the last thread's channels are moved back to end with D: the ones that it shares with the thread in
+// front are worked out and stored twice, the same.  (Measured before, a channel a thread: T 4096, B 8, D 2047, bf16, K 4, both
+// passes, 261 us.)
 // Frames are taken K at a time, so that a frame's place in the window (s mod K) is known when the code is compiled and nothing
 // is moved from register to register.
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p) {
-    const int d = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
+    const int dg = (blockIdx.x * 64 + (threadIdx.x & 63)) * V, d = min(dg, p.D - V);
     const int b = blockIdx.z;
     constexpr int RUN = conv_run(K, 16);
     const int s0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * RUN;
-    if (d >= p.D) return;
+    if (dg >= p.D) return;
     const int len = row_len(p.lens, b, p.T);
     const int s1 = min(s0 + RUN, p.T);
     T* out = (T*)p.out + b * p.o_sb + d;
@@ -75,7 +78,7 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p) {
                 for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][e], win[(j + k) % K][e], a);
                 y[e] = p.act ? silu_(a) : a;
             }
-            stv<T, V>(out + (p.reverse ? len - 1 - s : s) * p.o_st, y);
+            stu<T, V>(out + (p.reverse ? len - 1 - s : s) * p.o_st, y);
         };
         // whole windows: the next one is on its way while one is worked on
         int s = s0;
@@ -106,14 +109,14 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p) {
         }
     }
     const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int s = max(s0, len); s < s1; ++s) stv<T, V>(out + s * p.o_st, zero);
+    for (int s = max(s0, len); s < s1; ++s) stu<T, V>(out + s * p.o_st, zero);
     // the carried state: the inputs at the last K-1 walking positions (positions in front of the row stay state rows)
     if (p.state_out && s0 == 0) {
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) {
             float v[V];
             load_x<T, V, K>(p, len - (K - 1) + k, len, b, d, v);
-            stv<T, V>((T*)p.state_out + ((size_t)k * p.B + b) * p.D + d, v);
+            stu<T, V>((T*)p.state_out + ((size_t)k * p.B + b) * p.D + d, v);
         }
     }
 }
@@ -124,11 +127,11 @@ template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p) {
     __shared__ float sm[3][K + 1][64 * V];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const int d = (blockIdx.x * 64 + lane) * V;
+    const int dg = (blockIdx.x * 64 + lane) * V, d = min(dg, p.D - V);
     const int b = blockIdx.z;
     constexpr int RUN = conv_run(K, 32);
     const int s0 = (blockIdx.y * 4 + wv) * RUN;
-    const bool on = d < p.D;
+    const bool on = dg < p.D;
     const int len = row_len(p.lens, b, p.T);
     const int s1 = min(s0 + RUN, p.T);
     float dw[K + 1][V];
@@ -177,12 +180,12 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p) {
             const int r = s - (len - (K - 1));     // this position's row of the carried-out state
             if (p.dstate_out && r >= 0) {
                 float ds[V];
-                ldv<T, V>((const T*)p.dstate_out + ((size_t)r * p.B + b) * p.D + d, ds);
+                ldu<T, V>((const T*)p.dstate_out + ((size_t)r * p.B + b) * p.D + d, ds);
 #pragma unroll
                 for (int e = 0; e < V; ++e) o[e] += ds[e];
             }
-            if (s >= 0) stv<T, V>((T*)p.dx + ((size_t)(p.reverse ? len - 1 - s : s) * p.B + b) * p.D + d, o);
-            else if (p.dstate) stv<T, V>((T*)p.dstate + ((size_t)(s + K - 1) * p.B + b) * p.D + d, o);
+            if (s >= 0) stu<T, V>((T*)p.dx + ((size_t)(p.reverse ? len - 1 - s : s) * p.B + b) * p.D + d, o);
+            else if (p.dstate) stu<T, V>((T*)p.dstate + ((size_t)(s + K - 1) * p.B + b) * p.D + d, o);
         };
         // whole windows: the next one is on its way while one is worked on
         int q = s0;
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p) {
                 if (q + j < len) {
                     float g[V];
                     load_x<T, V, K>(p, q + j, len, b, d, win[(j + K - 1) % K]);
-                    ldv<T, V>(pdo + (p.reverse ? len - 1 - q - j : q + j) * p.do_st, g);
+                    ldu<T, V>(pdo + (p.reverse ? len - 1 - q - j : q + j) * p.do_st, g);
                     gradient(j, g, q + j < own);
                 } else {
 #pragma unroll
@@ -231,7 +234,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p) {
     }
     if (on) {
         const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        for (int s = max(s0, len); s < s1; ++s) stv<T, V>((T*)p.dx + ((size_t)s * p.B + b) * p.D + d, zero);
+        for (int s = max(s0, len); s < s1; ++s) stu<T, V>((T*)p.dx + ((size_t)s * p.B + b) * p.D + d, zero);
     }
     // four runs of a workgroup are joined in order
     if (wv) {
@@ -296,31 +299,32 @@ static int run_groups(int T, int K, int n) {
                                    CONV_K(5, __VA_ARGS__) CONV_K(6, __VA_ARGS__) CONV_K(7, __VA_ARGS__) \
                                    CONV_K(8, __VA_ARGS__) default: return ASR_ERR_LIMIT; }
 
+// Bytes a thread: 16 forward (8 of a 16-bit type from 6 taps on, whose two windows would not leave registers for two waves per SIMD), 8
+// backward: there two windows of x and dout on their way, the windows of x and dpre and the parts of dw are 150 registers at 8
+// bytes, 250 at 16 (one wave per SIMD); 4 of a 16-bit type from 6 taps on.  Measured for both passes: backward 8 / 16 / 4 bytes, T 4096,
+// B 16, D 2048, bf16, K 4: 339 / 398 / 344 us; T 2262, B 16, D 1024, f32: 135 / 139 / 138 us; the rule for 6 taps and more, T 4096,
+// B 8, D 2048, bf16: K 6 205 -> 180 us, K 7 214 -> 211, K 8 366 -> 246.
+// Few channels leave most lanes of a wave without any at that width: one value a thread below 24 (32) threads' worth.  T 4096, B 8,
+// bf16, K 4, D 99: 35 us at full width, 27 so; D 199: 37.5 and 35.3 (B 64: 166 and 226).
 template <typename T>
 static int conv_fwd_t(const ConvArgs& p, int k_, hipStream_t stream) {
-    constexpr int VW = 16 / sizeof(T);
-    const bool vec = p.D % VW == 0 && al16(p.x) && al16(p.out) && al16(p.state) && al16(p.state_out) &&
-                     stride_ok(p.x_st, VW) && stride_ok(p.x_sb, VW) && stride_ok(p.o_st, VW) && stride_ok(p.o_sb, VW);
-    const int V = vec ? VW : 1;
-    const dim3 grid((p.D + 64 * V - 1) / (64 * V), run_groups(p.T, k_, 16), p.B);
-    if (vec) { CONV_KS(hipLaunchKernelGGL((conv_fwd_kernel<T, VW, K>), grid, dim3(256), 0, stream, p)) }
-    else { CONV_KS(hipLaunchKernelGGL((conv_fwd_kernel<T, 1, K>), grid, dim3(256), 0, stream, p)) }
+    CONV_KS(
+        constexpr int VW = (sizeof(T) == 2 && K > 5 ? 8 : 16) / sizeof(T);
+        const bool vec = p.D >= 24 * VW; const int V = vec ? VW : 1;
+        const dim3 grid((p.D + 64 * V - 1) / (64 * V), run_groups(p.T, K, 16), p.B);
+        if (vec) hipLaunchKernelGGL((conv_fwd_kernel<T, VW, K>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((conv_fwd_kernel<T, 1, K>), grid, dim3(256), 0, stream, p);)
     ASR_CHECK_LAUNCH();
     return ASR_OK;
 }
-// 8 bytes a thread here: two windows of x and dout on their way, the windows of x and dpre and the parts of dw are 150 registers
-// at 8 bytes, 250 at 16 (one wave per SIMD).  Measured for both passes, 8 / 16 / 4 bytes: T 4096, B 16, D 2048, bf16, K 4: 339 /
-// 398 / 344 us; T 2262, B 16, D 1024, f32: 135 / 139 / 138 us.
 template <typename T>
 static int conv_bwd_t(const ConvArgs& p, int k_, hipStream_t stream) {
-    constexpr int VW = 8 / sizeof(T);
-    const bool vec = p.D % VW == 0 && al(p.x, 8) && al(p.dout, 8) && al(p.state, 8) && al(p.dstate_out, 8) && al(p.dx, 8) &&
-                     al(p.dstate, 8) && stride_ok(p.x_st, VW) && stride_ok(p.x_sb, VW) && stride_ok(p.do_st, VW) &&
-                     stride_ok(p.do_sb, VW);
-    const int V = vec ? VW : 1;
-    const dim3 grid((p.D + 64 * V - 1) / (64 * V), run_groups(p.T, k_, 32), p.B);
-    if (vec) { CONV_KS(hipLaunchKernelGGL((conv_bwd_kernel<T, VW, K>), grid, dim3(256), 0, stream, p)) }
-    else { CONV_KS(hipLaunchKernelGGL((conv_bwd_kernel<T, 1, K>), grid, dim3(256), 0, stream, p)) }
+    CONV_KS(
+        constexpr int VW = (sizeof(T) == 2 && K > 5 ? 4 : 8) / sizeof(T);
+        const bool vec = p.D >= 32 * VW; const int V = vec ? VW : 1;
+        const dim3 grid((p.D + 64 * V - 1) / (64 * V), run_groups(p.T, K, 32), p.B);
+        if (vec) hipLaunchKernelGGL((conv_bwd_kernel<T, VW, K>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((conv_bwd_kernel<T, 1, K>), grid, dim3(256), 0, stream, p);)
     ASR_CHECK_LAUNCH();
     return ASR_OK;
 }

@@ -8,27 +8,6 @@
 // tensors, some of them still in the Infinity Cache), backward 81 us (4.6 TB/s of 0.37 GB) and 5 for the parts of dw.
 #include "seq_common.h"
 
-// V values from any address that suits T: gfx950 takes 16 bytes at a time from there, and a wave's 1 KiB touches one line more.
-template <typename T, int V> struct AnyV { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
-template <typename T> struct AnyV<T, 1> { typedef T type; };
-template <typename T, int V> __device__ __forceinline__ void ldu(const T* p, float* o) {
-    const typename AnyV<T, V>::type v = *(const typename AnyV<T, V>::type*)p;
-    if constexpr (V == 1) o[0] = (float)v;
-    else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = (float)v[e];
-    }
-}
-template <typename T, int V> __device__ __forceinline__ void stu(T* p, const float* o) {
-    typename AnyV<T, V>::type v;
-    if constexpr (V == 1) v = (T)o[0];
-    else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = (T)o[e];
-    }
-    *(typename AnyV<T, V>::type*)p = v;
-}
-
 // A row is walked in groups of V columns, a lane to a group.  Where n is no multiple of V the last group is moved back to end with
 // the row: its first `skip` columns are the group's in front of it too, are left out of its sums, and are stored twice, the same.
 // Lanes behind the row stand on that group too (skip >= V: all of it) and store nothing: no branch between a row's loads.

@@ -34,6 +34,27 @@ template <typename T, int V> __device__ __forceinline__ void stv(T* p, const flo
     }
 }
 
+// V values from any address that suits T: gfx950 takes 16 bytes at a time from there, and a wave's 1 KiB touches one line more than it has to.
+template <typename T, int V> struct AnyV { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
+template <typename T> struct AnyV<T, 1> { typedef T type; };
+template <typename T, int V> __device__ __forceinline__ void ldu(const T* p, float* o) {
+    const typename AnyV<T, V>::type v = *(const typename AnyV<T, V>::type*)p;
+    if constexpr (V == 1) o[0] = (float)v;
+    else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = (float)v[e];
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void stu(T* p, const float* o) {
+    typename AnyV<T, V>::type v;
+    if constexpr (V == 1) v = (T)o[0];
+    else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = (T)o[e];
+    }
+    *(typename AnyV<T, V>::type*)p = v;
+}
+
 // e^-|v| in (0, 1]: the argument's product with log2 e in two floats, the rest as a first-order correction.  Finite for
 // every v (a NaN becomes e^-110): the functions below carry v itself on, and with it infinities and NaN.
 __device__ __forceinline__ float exp_neg_abs_(float v) {

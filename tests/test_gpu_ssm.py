@@ -72,6 +72,12 @@ CONV = [  # T, B, D, K, type, layout, lens, reverse, state, bias, act
     (300, 2, 520, 4, 'f32', 'c', [300, 299], False, True, True, 'silu'),
     (64, 2, 40, 6, 'f16', 'c', [2, 64], False, True, True, 'silu'),
     (0, 2, 8, 4, 'f32', 'c', None, False, True, True, 'silu'),
+    # a last thread whose channels are moved back to end with D, at either width of either pass
+    (150, 2, 203, 4, 'bf16', 'odd', [150, 31], True, True, True, 'silu'),
+    (70, 3, 131, 8, 'f16', 'half', [70, 0, 1], False, True, True, 'silu'),
+    (90, 2, 130, 6, 'f32', 'odd', [90, 6], False, True, True, 'silu'),
+    (40, 2, 67, 2, 'f32', 'c', None, True, True, True, None),
+    (50, 2, 515, 3, 'f16', 'bt', [50, 50], True, True, False, 'silu'),
 ]
 
 
