@@ -39,13 +39,15 @@ __device__ __forceinline__ float sum16(const float (&v)[16], int lane) {
     return z + dpp<0x4E>(z);                                         // quad_perm [2,3,0,1]
 }
 
+// EDGE: a group's channels are no multiple of 64, so that its last workgroup has idle lanes.  (With the tests for them in every kernel
+// the other sizes lose 5 %; a path without them for the workgroups that have none costs the loop its registers.)
 // PRE: the adjoint a chunk hands to the one in front of it when nothing comes in from behind, and its sum of delta.
 // Behind a tile's first adjoints, when the first of its states have left their registers, the tile in front of it is called from
 // memory; it goes into the input buffers behind the tile's first barrier, beside the joins.  (Called a tile
 // earlier, as the forward pass does, it costs 30 registers where they are scarcest: one wave per SIMD less, or spills; called
 // half way through the adjoints the spills are 28 registers, and T 2048, B 16, D 2048, bf16 takes 937 us instead of 886; one input
 // buffer instead of two, 840.)
-template <typename TY, int SPL, int NB, bool PRE>
+template <typename TY, int SPL, int NB, bool PRE, bool EDGE>
 __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
     constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RS = 8 / SPL;    // RS frames give sixteen sums
     constexpr int RB = (TS * NP + 255) / 256;
@@ -58,6 +60,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
     __shared__ float s_y[PRE ? 1 : 4][PRE ? 1 : TS][64];
     __shared__ float s_bc[PRE ? 1 : TS * 2 * NP];
     const Place q = sscan_place(p);
+    const bool on = !EDGE || q.on;
     const int tid = threadIdx.x, lane = q.lane, w = q.w;
     if (PRE && (q.k == 0 || q.t0 >= q.t1)) return;
     // without a gate x stands in for z and the gate's factors are replaced: no branch in the loop
@@ -90,7 +93,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
         }
     }
     // idle lanes stand on a real channel: whatever it holds, they must give zeros to the sums dB and dC
-    if (!q.on) {
+    if (!on) {
 #pragma unroll
         for (int m = 0; m < NB; ++m)
 #pragma unroll
@@ -116,10 +119,10 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool ok = FULL || tile * TS + w * 4 + i < q.len;
+            const bool live = ok && on;                 // an idle lane's dy and delta x are zero: nothing of it in dB and dC
             const float v = (float)ldt[i] + bias, g = ok ? (float)lg[i] : 0.f;
             const float u = exp_neg_abs_(v), sp = softplus_from_(v, u), sv = sigmoid_from_(v, u);
-            const bool live = ok && (FULL || q.on);
-            const float de = live ? (soft ? sp : v) : 0.f;
+            const float de = ok ? (soft ? sp : v) : 0.f;
             ns[i] = ok ? (soft ? sv : 1.f) : 0.f;
             const float z = ok ? (float)lz[i] : 0.f, sg = sigm_(z);
             const float dy = gated ? g * z * sg : g;
@@ -140,11 +143,11 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
         unsigned at = d * 4u;
 #pragma unroll
         for (int j = 0; j < SPL; ++j) {
-            o[j] = q.on ? *(const float*)(ck + at) : 0.f;
+            o[j] = on ? *(const float*)(ck + at) : 0.f;
             ck += (size_t)k->D * 4;
         }
     };
-    // a tile; FULL: it and the one in front of it hold valid frames alone, and all lanes have a channel
+    // a tile; FULL: it and the one in front of it hold valid frames alone
     const auto walk = [&](int tile, auto full) {
         constexpr bool FULL = decltype(full)::value;
         const int half = PRE ? (q.t1 - 1 - tile) & 1 : 0, sb = tile * TS;
@@ -255,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
         const KArgs k = kargs();
         const int T = k->T, rev = k->reverse;
         const long long ost = (long long)k->B * k->D, orow = (long long)q.b * k->D;
-        if (FULL || q.on) {
+        if (on) {
             store_rows<FULL>((TY*)k->dx + orow, ost, s0, q.len, T, rev, off, ox);
             store_rows<FULL>((TY*)k->ddt + orow, ost, s0, q.len, T, rev, off, odt);
             if (gated) store_rows<FULL>((TY*)k->dz + orow, ost, s0, q.len, T, rev, off, oz);
@@ -279,11 +282,10 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
     int tile = q.t1 - 1;
     for (; tile >= q.t0 && (tile * TS + TS > q.len); --tile) walk(tile, Flag<false>{});
     // (a chunk's first tile calls for the one in front of it, which is thrown away)
-    if (__builtin_amdgcn_ballot_w64(q.on) == ~0ull)
-        for (; tile >= max(q.t0, 1); --tile) walk(tile, Flag<true>{});
+    for (; tile >= max(q.t0, 1); --tile) walk(tile, Flag<true>{});
     for (; tile >= q.t0; --tile) walk(tile, Flag<false>{});
     if (PRE) {
-        if (!q.on) return;
+        if (!on) return;
 #pragma unroll
         for (int m = 0; m < NB; ++m)
 #pragma unroll
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
     }
     // padding, the parts of the parameter gradients, the gradient of the first state
     const int send = min(p.T, (q.t0 + p.tpc) * TS);
-    if (q.on) {
+    if (on) {
         for (int s = max(q.nt, q.t0) * TS + w; s < send; s += 4) {
             const size_t o = ((size_t)s * p.B + q.b) * p.D + d;
             stf((TY*)p.dx + o, 0.f);
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
         }
     }
     const size_t row = (size_t)q.k * p.B + q.b;
-    if (q.on) {
+    if (on) {
 #pragma unroll
         for (int m = 0; m < NB; ++m)
 #pragma unroll
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
     s_dy[0][w][lane] = accD;
     s_dy[0][4 + w][lane] = accb;
     __syncthreads();
-    if (w < 2 && q.on) {
+    if (w < 2 && on) {
         const float* v = &s_dy[0][w * 4][lane];
         (w ? p.part_b : p.part_d)[row * p.D + d] = (v[0] + v[64]) + (v[128] + v[192]);
     }
@@ -392,11 +394,16 @@ static BwdWs bwd_ws(int T, int B, int D, int N, int G) {
 }
 size_t sscan_bwd_ws(int T, int B, int D, int N, int G) { return bwd_ws(T, B, D, N, G).total; }
 
+template <typename TY, int SPL, int NB, bool EDGE>
+static void launch_bwd_e(const SscanArgs& p, hipStream_t stream) {
+    const dim3 grid(p.G * p.tpg, p.B, p.S);
+    if (p.S > 1) hipLaunchKernelGGL((sstate_bwd_kernel<TY, SPL, NB, true, EDGE>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((sstate_bwd_kernel<TY, SPL, NB, false, EDGE>), grid, dim3(256), 0, stream, p);
+}
 template <typename TY, int SPL, int NB>
 static void launch_bwd(const SscanArgs& p, hipStream_t stream) {
-    if (p.S > 1)
-        hipLaunchKernelGGL((sstate_bwd_kernel<TY, SPL, NB, true>), dim3(p.G * p.tpg, p.B, p.S), dim3(256), 0, stream, p);
-    hipLaunchKernelGGL((sstate_bwd_kernel<TY, SPL, NB, false>), dim3(p.G * p.tpg, p.B, p.S), dim3(256), 0, stream, p);
+    if (p.dpg % 64) launch_bwd_e<TY, SPL, NB, true>(p, stream);
+    else launch_bwd_e<TY, SPL, NB, false>(p, stream);
 }
 template <typename TY>
 static void launch_bwd_t(const SscanArgs& p, const asr_sscan_desc* d, hipStream_t stream) {

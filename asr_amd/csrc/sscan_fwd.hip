@@ -98,7 +98,8 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
         if (FULL || q.on) store_rows<FULL>(po, p.o_st, tile * TS + w * 4, q.len, p.T, p.reverse, off, y);
     };
     // a tile, and behind it the tile in front (`prev`), so that its joins and stores run beside the walk.  FULL: it, the next
-    // and the one after that, and the one in front, hold valid frames alone, and all lanes have a channel
+    // and the one after that, and the one in front, hold valid frames alone (a lane without a channel of its own does what the last
+    // one with a channel does, its stores included)
     const auto walk = [&](int tile, auto full, auto prev) {
         constexpr bool FULL = decltype(full)::value;
         const int half = (tile - q.t0) & 1;
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
         __syncthreads();
     }
     // (a chunk's last tiles call for the next chunk's first two: valid frames, thrown away)
-    const int clear = __builtin_amdgcn_ballot_w64(q.on) == ~0ull ? min(q.t1, q.len / TS - 2) : 0;
+    const int clear = min(q.t1, q.len / TS - 2);
     int tile = q.t0;
     if (tile < clear) walk(tile++, Flag<true>{}, Flag<false>{});
     else if (tile < q.t1) walk(tile++, Flag<false>{}, Flag<false>{});
@@ -217,16 +218,24 @@ __global__ __launch_bounds__(256) void sscan_step_kernel(SscanArgs p) {
 }
 
 // ---------------------------------------------------------------- C entries
-// Chunks of time.  One while batch rows x channel tiles give every CU two workgroups (512): a second pass over the chunks then
-// only costs (T 2048, B 16, D 2048, bf16, 512 workgroups: forward 379 us with one chunk, 482 with two; backward 1043, 1249).
-// With fewer, forward as many chunks as fill the three workgroups that a CU's LDS holds (768; T 1207, B 16, D 1024, f32, ragged, 256
-// workgroups: 2 / 3 / 4 / 6 / 8 chunks: 183 / 151 / 155 / 153 / 148 us; T 16384, B 1, D 2048, bf16, 32 workgroups: 8 / 16 / 24 / 32 /
-// 64 chunks: 453 / 310 / 277 / 287 / 286 us), backward four rounds of the two it holds (2048), which evens out ragged rows (the
-// first case: 4 / 6 / 8 / 10 / 12 chunks: 315 / 308 / 294 / 310 / 309 us), of at least four tiles each.
+// Chunks of time, where batch rows x channel tiles (`wgs` workgroups) leave the chip idle: a first pass over the chunks costs two
+// thirds of a forward pass and 28 % of a backward one.  Measured at 1024 frames, bf16, 16 states, us:
+//   workgroups        128   192   256   320   384   448   480   512   544   640   704
+//   forward, one      129   130   130   164   166   167   167   167   216   218   220
+//     768 / wgs        79   111   129   186   188    as one
+//   backward, one     321   325   326   436   438   441   442   444   687   691   693
+//     chunks          169   239   305   387   435   530   541   547   618   684   753    (2048 / wgs, from 512 on 4)
+// So forward below 256 as many as make the three workgroups of a CU; backward up to 400 four rounds of the two that a CU holds, which
+// also evens out ragged rows (256 workgroups, T 1207, f32, 4 / 6 / 8 / 10 / 12 chunks: 315 / 308 / 294 / 310 / 309 us), and four chunks
+// where a second round of workgroups would be nearly empty.  (Ragged rows gain less from one chunk: 480 workgroups 417 us, six chunks
+// 386; 544: a step 2 % slower with four.)  A single row (32 workgroups, T 16384): 8 / 16 / 24 / 32 / 64 chunks
+// 453 / 310 / 277 / 287 / 286 us.  At least four tiles each.
 int sscan_chunks(int T, int B, int D, int G, int backward) {
     const long long wgs = (long long)G * ((D / G + 63) / 64) * B;
     const int nt = sscan_tiles(T);
-    long long S = wgs > 0 && wgs < 512 ? (backward ? 2048 : 768) / wgs : 1;
+    long long S = 1;
+    if (wgs > 0 && wgs < (backward ? 401 : 256)) S = (backward ? 2048 : 768) / wgs;
+    else if (backward && wgs > 512 && wgs <= 640) S = 4;
     if (S > nt / 4) S = nt / 4;
     if (S > 64) S = 64;
     return S < 1 ? 1 : (int)S;
