@@ -5,7 +5,7 @@
 // in registers (16 frames x states, with a), then the adjoint runs back over them.
 //
 // Bound by the vector unit: 14 issue slots per (frame, channel, state) and 4.4 for the sums over lanes, about 110 per (frame,
-// channel).  Measured at T 2048, B 16, D 2048, 16 states, bf16: 840 us, and 31 for the sums over workgroups; those slots are 505 us,
+// channel).  Measured at T 2048, B 16, D 2048, 16 states, bf16: 855 us, and 31 for the sums over workgroups; those slots are 505 us,
 // the bytes of both passes together 230 us; counters: 83 % of all SIMD cycles issue a vector instruction.
 #include "sscan.h"
 
@@ -40,13 +40,13 @@ __device__ __forceinline__ float sum16(const float (&v)[16], int lane) {
 }
 
 // EDGE: a group's channels are no multiple of 64, so that its last workgroup has idle lanes.  (With the tests for them in every kernel
-// the other sizes lose 5 %; a path without them for the workgroups that have none costs the loop its registers.)
+// the other sizes lose 5 %; three loops in one kernel cost them 18 %, by registers.)
 // PRE: the adjoint a chunk hands to the one in front of it when nothing comes in from behind, and its sum of delta.
 // Behind a tile's first adjoints, when the first of its states have left their registers, the tile in front of it is called from
 // memory; it goes into the input buffers behind the tile's first barrier, beside the joins.  (Called a tile
 // earlier, as the forward pass does, it costs 30 registers where they are scarcest: one wave per SIMD less, or spills; called
 // half way through the adjoints the spills are 28 registers, and T 2048, B 16, D 2048, bf16 takes 937 us instead of 886; one input
-// buffer instead of two, 840.)
+// buffer instead of two, 840 to 855.)
 template <typename TY, int SPL, int NB, bool PRE, bool EDGE>
 __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
     constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RS = 8 / SPL;    // RS frames give sixteen sums

@@ -225,7 +225,7 @@ __global__ __launch_bounds__(256) void sscan_step_kernel(SscanArgs p) {
 //     768 / wgs        79   111   129   186   188    as one
 //   backward, one     321   325   326   436   438   441   442   444   687   691   693
 //     chunks          169   239   305   387   435   530   541   547   618   684   753    (2048 / wgs, from 512 on 4)
-// So forward below 256 as many as make the three workgroups of a CU; backward up to 400 four rounds of the two that a CU holds, which
+// So forward up to 256 as many as make the three workgroups of a CU (at 256 and T 1207, f32, ragged: 168 us with one, 152 with three); backward up to 400 four rounds of the two that a CU holds, which
 // also evens out ragged rows (256 workgroups, T 1207, f32, 4 / 6 / 8 / 10 / 12 chunks: 315 / 308 / 294 / 310 / 309 us), and four chunks
 // where a second round of workgroups would be nearly empty.  (Ragged rows gain less from one chunk: 480 workgroups 417 us, six chunks
 // 386; 544: a step 2 % slower with four.)  A single row (32 workgroups, T 16384): 8 / 16 / 24 / 32 / 64 chunks
@@ -234,7 +234,7 @@ int sscan_chunks(int T, int B, int D, int G, int backward) {
     const long long wgs = (long long)G * ((D / G + 63) / 64) * B;
     const int nt = sscan_tiles(T);
     long long S = 1;
-    if (wgs > 0 && wgs < (backward ? 401 : 256)) S = (backward ? 2048 : 768) / wgs;
+    if (wgs > 0 && wgs < (backward ? 401 : 257)) S = (backward ? 2048 : 768) / wgs;
     else if (backward && wgs > 512 && wgs <= 640) S = 4;
     if (S > nt / 4) S = nt / 4;
     if (S > 64) S = 64;
