@@ -6,7 +6,7 @@
 //
 // Bound by the vector unit: 14 issue slots per (frame, channel, state) and 4.4 for the sums over lanes, about 110 per (frame,
 // channel).  Measured at T 2048, B 16, D 2048, 16 states, bf16: 855 us, and 31 for the sums over workgroups; those slots are 505 us,
-// the bytes of both passes together 230 us; counters: 83 % of all SIMD cycles issue a vector instruction.
+// the bytes of both passes together 230 us; counters: 81 % of all SIMD cycles issue a vector instruction.
 #include "sscan.h"
 
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
