@@ -208,7 +208,8 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
                             v[i * 2 * SPL + j] = dh * du.y;
                             v[i * 2 * SPL + SPL + j] = dy * h[t][j];
                             r[m][j] = a[t][j] * dh;
-                            const float qq = r[m][j] * (t ? h[t - 1][j] : h0[j]);
+                            // padding: a is 1 and the last state and its gradient meet as they do in no valid frame
+                            const float qq = (FULL || sb + t < q.len) ? r[m][j] * (t ? h[t - 1][j] : h0[j]) : 0.f;
                             s2 = __builtin_fmaf(qq, A2[m][j], s2);
                             da[j] = __builtin_fmaf(qq, du.x, da[j]);
                             s1 = __builtin_fmaf(dh, s_B[half][e], s1);
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
             const float2 a = s_s[0][t][lane], b = s_s[1][t][lane], c = s_s[2][t][lane], e = s_s[3][t][lane];
             const float s1 = (a.x + b.x) + (c.x + e.x), s2 = (a.y + b.y) + (c.y + e.y);
             ox[i] = __builtin_fmaf(de[i], s1, Dk * dy[i]);
-            odt[i] = __builtin_fmaf(rx[i], s1, s2 * LN2) * rs[i];
+            odt[i] = (FULL || s0 + i < q.len) ? __builtin_fmaf(rx[i], s1, s2 * LN2) * rs[i] : 0.f;
             oz[i] = rg[i] * (((s_y[0][t][lane] + s_y[1][t][lane]) + (s_y[2][t][lane] + s_y[3][t][lane])) + Dk * rx[i]);
             accD = __builtin_fmaf(dy[i], rx[i], accD);     // frames of the padding give zeros
             accb += odt[i];
