@@ -68,7 +68,7 @@ __device__ __forceinline__ Place sscan_place(const SscanArgs& p) {
     return q;
 }
 
-// A log2(e), finite below: a padding frame's delta of zero must leave exp(delta A) at 1 whatever the rate is.
+// A log2(e), finite below: a delta of zero (a padding frame's, or a valid one's) must leave exp(delta A) at 1 for a rate of -inf too.
 __device__ __forceinline__ float rate2(float A) {
     const float v = A * LOG2E;
     return v < -3.0e38f ? -3.0e38f : v;

@@ -197,13 +197,13 @@ __global__ __launch_bounds__(256) void sscan_step_kernel(SscanArgs p) {
         const f32x4 av = *(const f32x4*)(A + n0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            hv[e] = __builtin_fmaf(__builtin_amdgcn_exp2f(av[e] * LOG2E * de), hv[e], u * ldf(pB + n0 + e));
+            hv[e] = __builtin_fmaf(__builtin_amdgcn_exp2f(rate2(av[e]) * de), hv[e], u * ldf(pB + n0 + e));
             y = __builtin_fmaf(ldf(pC + n0 + e), hv[e], y);
         }
         *(f32x4*)(h + n0) = hv;
     } else {
         for (int e = 0; e < m; ++e) {
-            const float v = __builtin_fmaf(__builtin_amdgcn_exp2f(A[n0 + e] * LOG2E * de), h[n0 + e], u * ldf(pB + n0 + e));
+            const float v = __builtin_fmaf(__builtin_amdgcn_exp2f(rate2(A[n0 + e]) * de), h[n0 + e], u * ldf(pB + n0 + e));
             h[n0 + e] = v;
             y = __builtin_fmaf(ldf(pC + n0 + e), v, y);
         }

@@ -65,3 +65,28 @@ def test_gradient_of_a_large_state_in_front_of_padding(D, N):
     dh[..., 0] = 2e19 * sign(B, D)
     gradients(a, dict(dt_bias=torch.zeros(D).cuda()), [37, 21], rn(g, T, B, D), dh, ('x', 'dt', 'A', 'B', 'C', 'dt_bias'),
               dict(B=1e30))
+
+
+@pytest.mark.parametrize('softplus', [True, False])
+@pytest.mark.parametrize('rate', [float('-inf'), -3e38])
+@pytest.mark.parametrize('N', [16, 5])
+def test_a_frame_without_delta_leaves_the_state_alone_at_any_rate(N, rate, softplus):
+    """single frames and the sequence: delta is exactly zero in every third frame (softplus(-200), or dt = 0), where a decay of
+    any rate has no time to act"""
+    from asr_amd import ops
+    T, B, D = 12, 3, 64
+    a, opt = scan_inputs(gen(51), T, B, D, N, 1, torch.float32)
+    opt['dt_bias'] = None
+    a['dt'] = a['dt'].abs() + 0.1
+    a['dt'][::3] = -200.0 if softplus else 0.0
+    a['A'][:, 0] = rate
+    kw = dict(softplus=softplus)
+    out, h, _ = ops.selective_scan_fwd(*a.values(), **opt, **kw)
+    st = opt['h0'].clone()
+    steps = torch.stack([ops.selective_scan_step(st, a['x'][t], a['dt'][t], a['A'], a['Bm'][t], a['Cm'][t], D=opt['D'],
+                                                 z=opt['z'][t], **kw) for t in range(T)])
+    ra = {k: R.leaf(v.clamp(min=-3e38) if k == 'A' else v, False) for k, v in a.items()}
+    ro, rh = R.scan(*ra.values(), **{k: R.leaf(v, False) for k, v in opt.items()}, **kw)
+    k = 8 * T + 2 * N + 32
+    for name, got, ref in (('out', out, ro), ('h', h, rh), ('steps', steps, ro), ('h after steps', st, rh)):
+        R.close(got, ref, k, name)
