@@ -68,10 +68,10 @@ __device__ __forceinline__ Place sscan_place(const SscanArgs& p) {
     return q;
 }
 
-// A log2(e), finite below: a delta of zero (a padding frame's, or a valid one's) must leave exp(delta A) at 1 for a rate of -inf too.
+// A log2(e), finite: a delta of zero (a padding frame's, or a valid one's) must leave exp(delta A) at 1 whatever the rate is.
 __device__ __forceinline__ float rate2(float A) {
     const float v = A * LOG2E;
-    return v < -3.0e38f ? -3.0e38f : v;
+    return v < -3.0e38f ? -3.0e38f : v > 3.0e38f ? 3.0e38f : v;        // NaN stays
 }
 
 // h 2^k, a state carried over a whole chunk.  In three factors: of a state that grows (k > 0) 2^k may overflow where h 2^k does

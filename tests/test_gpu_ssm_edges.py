@@ -90,3 +90,24 @@ def test_a_frame_without_delta_leaves_the_state_alone_at_any_rate(N, rate, softp
     k = 8 * T + 2 * N + 32
     for name, got, ref in (('out', out, ro), ('h', h, rh), ('steps', steps, ro), ('h after steps', st, rh)):
         R.close(got, ref, k, name)
+
+
+@pytest.mark.parametrize('T', [20, 150])
+def test_a_growing_rate_above_the_range_of_its_product_with_log2_e(T):
+    """a rate of 3e38 over frames whose delta is exactly zero: nothing grows, in single frames, in the sequence, in its chunks of
+    time, in the padding and in the gradients"""
+    from asr_amd import ops
+    B, D, N = 2, 64, 8
+    lens = [T, T - 7]
+    a, opt = scan_inputs(gen(61), T, B, D, N, 1, torch.float32)
+    opt.update(z=None, dt_bias=torch.zeros(D).cuda())
+    a['dt'].fill_(-200.0)
+    a['A'][:, 0] = 3e38
+    do, dh = rn(gen(62), T, B, D), rn(gen(63), B, D, N) * 0.1
+    gradients(a, {k: v for k, v in opt.items() if v is not None}, lens, do, dh, ('x', 'C', 'D', 'h0'))
+    st = opt['h0'].clone()
+    got = ops.selective_scan_step(st, a['x'][0], a['dt'][0], a['A'], a['Bm'][0], a['Cm'][0], D=opt['D'])
+    assert torch.equal(st, opt['h0'])
+    ref, _ = R.scan(*[R.leaf(v[:1] if k != 'A' else v, False) for k, v in a.items()], D=R.leaf(opt['D'], False),
+                    h0=R.leaf(opt['h0'], False))
+    R.close(got, ref[0], 8 + 2 * N + 32, 'out')
