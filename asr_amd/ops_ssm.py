@@ -420,9 +420,12 @@ def clip_list(tensors, max_norm, eps=1e-7):
         _fail('tensors: none given')
     if not max_norm >= 0 or not eps >= 0:
         _fail('max_norm %r and eps %r must not be negative' % (max_norm, eps))
-    kinds = [_type('tensors[%d]' % i, t) for i, t in enumerate(tensors)]
+    kinds = [_DTYPES.get(t.dtype) if t.layout is torch.strided else None for t in tensors]
     dev = tensors[0].get_device()
     for i, t in enumerate(tensors):
+        if kinds[i] is None:
+            _type('tensors[%d]' % i, t)
+            _fail('tensors[%d]: %s, expected a strided tensor' % (i, t.layout))
         if t.get_device() != dev:
             _fail('tensors[%d]: on %s, unlike the others' % (i, t.device))
     _gpu(dev)

@@ -71,6 +71,10 @@ class ClippedGrads(object):
     def __init__(self, max_norm, epsilon):
         self.max_norm = float(max_norm); self.epsilon = float(epsilon)
 
+    def __iter__(self):
+        raise TypeError("these stand for the network's own gradients, which its updater scales; a list of gradients is scaled by "
+                        "itself if it holds float32, bfloat16 or float16 tensors of one GPU alone")
+
 
 class NormHandle(object):
     """Second return value of total_norm_constraint(return_norm=True): filled by the next update."""
@@ -89,13 +93,18 @@ def total_norm_constraint(tensor_vars=None, max_norm=0.0, epsilon=1e-7, return_n
     """libs/lasagne_libs/updates.py:781-855 (lasagne.updates.total_norm_constraint).  A list of GPU tensors (gradients held
     outside a network's flat buffer, such as those of asr_amd.ops.selective_scan_bwd) is clipped here and now: the list of the
     scaled tensors is returned, with the norm as a (1,) tensor if return_norm.  Anything else stands for the network's own
-    gradients, which the optimiser kernel scales when it reads them."""
+    gradients, which the optimiser kernel scales when it reads them: lists that ops.clip_list refuses too (other types, tensors on
+    several devices, a max_norm or an epsilon below zero)."""
+    cg = ClippedGrads(max_norm, epsilon)
     if isinstance(tensor_vars, (list, tuple)) and all(isinstance(t, torch.Tensor) for t in tensor_vars) and any(
             t.is_cuda for t in tensor_vars):
-        scaled, norm = ops.clip_list(tensor_vars, max_norm, epsilon)
-        scaled = ScaledGrads(scaled, max_norm, epsilon)
-        return (scaled, norm) if return_norm else scaled
-    cg = ClippedGrads(max_norm, epsilon)
+        try:
+            scaled, norm = ops.clip_list(tensor_vars, cg.max_norm, cg.epsilon)
+        except ValueError:                             # refused before anything was launched
+            pass
+        else:
+            scaled = ScaledGrads(scaled, max_norm, epsilon)
+            return (scaled, norm) if return_norm else scaled
     return (cg, NormHandle()) if return_norm else cg
 
 

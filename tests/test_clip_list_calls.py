@@ -1,0 +1,54 @@
+"""updates.total_norm_constraint as a call: what it takes for a list of gradients to clip and what for the network's own, what it
+returns, and what an updater keeps of it."""
+import numpy as np
+import pytest
+import torch
+
+from asr_amd import ops, updates
+
+
+class OnGpu(torch.Tensor):
+    is_cuda = True
+
+
+def on_gpu(*shape, dtype=torch.float32):
+    return torch.ones(*shape, dtype=dtype).as_subclass(OnGpu)
+
+
+def is_stand_in(tensors, *args):
+    """-> the result stands for the network's own gradients, as it does for any argument that is no list of GPU tensors"""
+    cg, handle = updates.total_norm_constraint(tensors, *args, return_norm=True)
+    assert type(updates.total_norm_constraint(tensors, *args)) is updates.ClippedGrads
+    step, _ = updates.adam(cg)
+    assert step.kind == 7 and step.clip is cg and cg.max_norm == float(args[0])
+    with pytest.raises(TypeError, match='own gradients'):
+        list(cg)
+    return type(cg) is updates.ClippedGrads and type(handle) is updates.NormHandle
+
+
+def test_lists_that_cannot_be_clipped_stand_for_the_network_as_before():
+    for bad in ([on_gpu(3, dtype=torch.float64)], [on_gpu(3), on_gpu(2, dtype=torch.int64)], (on_gpu(3), torch.ones(2))):
+        assert is_stand_in(bad, 1.0)
+    for max_norm in (-1.0, np.float32(-2.0)):
+        assert is_stand_in([on_gpu(3)], max_norm)
+    assert is_stand_in([on_gpu(3)], 1.0, -1e-7)
+    with pytest.raises(ValueError, match='strided'):
+        ops.clip_list([torch.ones(3).to_sparse()], 1.0)
+
+
+@pytest.mark.gpu
+def test_gpu_lists_that_cannot_be_clipped_stand_for_the_network_as_before():
+    t = torch.ones(3, device='cuda')
+    for bad in ([t.double()], [t, t.long()], [t, torch.ones(2)], [torch.ones(2), t], [t.to_sparse()]):
+        assert is_stand_in(bad, 1.0)
+    assert is_stand_in([t], -1.0)
+
+
+@pytest.mark.gpu
+def test_max_norm_is_taken_as_a_number():
+    """a numpy scalar or a tensor of one value, as before"""
+    t = torch.full((4,), 3.0, device='cuda')
+    want = updates.total_norm_constraint([t], 1.5)
+    for m in (np.float32(1.5), torch.tensor(1.5), torch.tensor([1.5], device='cuda')):
+        got = updates.total_norm_constraint([t], m)
+        assert torch.equal(got[0], want[0]) and got.max_norm == 1.5
