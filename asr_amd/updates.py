@@ -81,6 +81,15 @@ class NormHandle(object):
     value = None
 
 
+class ListNorm(torch.Tensor):
+    """The same for a list that has been clipped: the norm as a (1,) tensor on the list's GPU, and its .value read from there."""
+    __torch_function__ = torch._C._disabled_torch_function_impl
+
+    @property
+    def value(self):
+        return self.item()
+
+
 class ScaledGrads(list, ClippedGrads):
     """The scaled tensors of a list.  An updater that is given it, as the reference's scripts do, still finds how the network's
     own gradients are to be clipped."""
@@ -92,7 +101,7 @@ class ScaledGrads(list, ClippedGrads):
 def total_norm_constraint(tensor_vars=None, max_norm=0.0, epsilon=1e-7, return_norm=False):
     """libs/lasagne_libs/updates.py:781-855 (lasagne.updates.total_norm_constraint).  A list of GPU tensors (gradients held
     outside a network's flat buffer, such as those of asr_amd.ops.selective_scan_bwd) is clipped here and now: the list of the
-    scaled tensors is returned, with the norm as a (1,) tensor if return_norm.  Anything else stands for the network's own
+    scaled tensors is returned, with the norm as a (1,) tensor if return_norm (its .value is the number).  Anything else stands for the network's own
     gradients, which the optimiser kernel scales when it reads them: lists that ops.clip_list refuses too (other types, tensors on
     several devices, a max_norm or an epsilon below zero)."""
     cg = ClippedGrads(max_norm, epsilon)
@@ -104,7 +113,7 @@ def total_norm_constraint(tensor_vars=None, max_norm=0.0, epsilon=1e-7, return_n
             pass
         else:
             scaled = ScaledGrads(scaled, max_norm, epsilon)
-            return (scaled, norm) if return_norm else scaled
+            return (scaled, norm.as_subclass(ListNorm)) if return_norm else scaled
     return (cg, NormHandle()) if return_norm else cg
 
 

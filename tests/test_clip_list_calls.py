@@ -36,6 +36,18 @@ def test_lists_that_cannot_be_clipped_stand_for_the_network_as_before():
         ops.clip_list([torch.ones(3).to_sparse()], 1.0)
 
 
+def clip_on_the_cpu(monkeypatch):
+    monkeypatch.setattr(ops, 'clip_list', lambda tensors, max_norm, eps: ([t.as_subclass(torch.Tensor) + 1 for t in tensors], torch.full((1,), 2.5)))
+
+
+def test_norm_of_a_list_has_a_value_like_the_network_s(monkeypatch):
+    clip_on_the_cpu(monkeypatch)
+    _, handle = updates.total_norm_constraint(None, 1.0, return_norm=True)
+    assert handle.value is None
+    _, norm = updates.total_norm_constraint([on_gpu(3)], 1.0, return_norm=True)
+    assert norm.value == 2.5 and norm.shape == (1,) and type(norm.reshape(()) + 1) is torch.Tensor
+
+
 @pytest.mark.gpu
 def test_gpu_lists_that_cannot_be_clipped_stand_for_the_network_as_before():
     t = torch.ones(3, device='cuda')
@@ -52,3 +64,5 @@ def test_max_norm_is_taken_as_a_number():
     for m in (np.float32(1.5), torch.tensor(1.5), torch.tensor([1.5], device='cuda')):
         got = updates.total_norm_constraint([t], m)
         assert torch.equal(got[0], want[0]) and got.max_norm == 1.5
+    _, norm = updates.total_norm_constraint([t], 1.5, return_norm=True)
+    assert norm.is_cuda and norm.value == 6.0
