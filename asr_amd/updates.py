@@ -11,6 +11,7 @@ parameter / gradient buffers, and opt_params_dict exposes the same keys ('t_prev
 elementwise HIP kernel asr_opt_step; the state tensors are flat, like the parameters.
 """
 from collections import OrderedDict
+from collections.abc import Iterable
 
 import numpy as np
 import torch
@@ -73,7 +74,7 @@ class ClippedGrads(object):
 
     def __iter__(self):
         raise TypeError("these stand for the network's own gradients, which its updater scales; a list of gradients is scaled by "
-                        "itself if it holds float32, bfloat16 or float16 tensors of one GPU alone")
+                        "itself if it holds float32, bfloat16 or float16 tensors of one GPU (and None)")
 
 
 class NormHandle(object):
@@ -99,21 +100,28 @@ class ScaledGrads(list, ClippedGrads):
 
 
 def total_norm_constraint(tensor_vars=None, max_norm=0.0, epsilon=1e-7, return_norm=False):
-    """libs/lasagne_libs/updates.py:781-855 (lasagne.updates.total_norm_constraint).  A list of GPU tensors (gradients held
-    outside a network's flat buffer, such as those of asr_amd.ops.selective_scan_bwd) is clipped here and now: the list of the
-    scaled tensors is returned, with the norm as a (1,) tensor if return_norm (its .value is the number).  Anything else stands for the network's own
-    gradients, which the optimiser kernel scales when it reads them: lists that ops.clip_list refuses too (other types, tensors on
-    several devices, a max_norm or an epsilon below zero)."""
+    """libs/lasagne_libs/updates.py:781-855 (lasagne.updates.total_norm_constraint).  GPU tensors in a list or any other iterable
+    (gradients held outside a network's flat buffer, such as those of asr_amd.ops.selective_scan_bwd) are clipped here and now: the
+    list of the scaled tensors is returned (None, a parameter without a gradient, stays None), with the norm as a (1,) tensor if
+    return_norm (its .value is the number).  Anything else stands for the network's own gradients, which the optimiser kernel
+    scales when it reads them: lists that ops.clip_list refuses too (other types, tensors on several devices, a max_norm or an
+    epsilon below zero)."""
     cg = ClippedGrads(max_norm, epsilon)
-    if isinstance(tensor_vars, (list, tuple)) and all(isinstance(t, torch.Tensor) for t in tensor_vars) and any(
-            t.is_cuda for t in tensor_vars):
-        try:
-            scaled, norm = ops.clip_list(tensor_vars, cg.max_norm, cg.epsilon)
-        except ValueError:                             # refused before anything was launched
-            pass
-        else:
-            scaled = ScaledGrads(scaled, max_norm, epsilon)
-            return (scaled, norm.as_subclass(ListNorm)) if return_norm else scaled
+    if (isinstance(tensor_vars, Iterable) and not isinstance(tensor_vars, (torch.Tensor, np.ndarray, str, dict))
+            and type(tensor_vars) is not ClippedGrads):
+        every = list(tensor_vars)
+        there = [t for t in every if t is not None]
+        if all(isinstance(t, torch.Tensor) for t in there) and any(t.is_cuda for t in there):
+            try:
+                scaled, norm = ops.clip_list(there, cg.max_norm, cg.epsilon)
+            except ValueError:                             # refused before anything was launched
+                pass
+            else:
+                if len(there) < len(every):
+                    left = iter(scaled)
+                    scaled = [None if t is None else next(left) for t in every]
+                scaled = ScaledGrads(scaled, max_norm, epsilon)
+                return (scaled, norm.as_subclass(ListNorm)) if return_norm else scaled
     return (cg, NormHandle()) if return_norm else cg
 
 

@@ -48,6 +48,23 @@ def test_norm_of_a_list_has_a_value_like_the_network_s(monkeypatch):
     assert norm.value == 2.5 and norm.shape == (1,) and type(norm.reshape(()) + 1) is torch.Tensor
 
 
+@pytest.mark.parametrize('kind', [list, tuple, iter, lambda ts: (t for t in ts), lambda ts: dict(enumerate(ts)).values()])
+def test_gradients_in_any_iterable_and_parameters_without_one(kind, monkeypatch):
+    clip_on_the_cpu(monkeypatch)
+    got, norm = updates.total_norm_constraint(kind([None, on_gpu(3), None, on_gpu(2), None]), 1.0, return_norm=True)
+    assert type(got) is updates.ScaledGrads and len(got) == 5 and got[0] is got[2] is got[4] is None
+    assert torch.equal(got[1], torch.full((3,), 2.0)) and torch.equal(got[3], torch.full((2,), 2.0)) and norm.value == 2.5
+    assert type(updates.total_norm_constraint(kind([on_gpu(1)]), 1.0)) is updates.ScaledGrads
+    once = updates.ScaledGrads([on_gpu(1)], 1.0, 1e-7)                  # clipped again
+    assert torch.equal(updates.total_norm_constraint(once, 1.0)[0], torch.full((1,), 2.0))
+
+
+def test_what_holds_no_gpu_tensor_stands_for_the_network_as_before():
+    for own in (None, [], [None], (), 'grads', np.zeros(3), torch.zeros(3), on_gpu(3), {'w': on_gpu(3)}, [np.zeros(3)], [torch.zeros(3), None],
+                iter([np.zeros(3)]), updates.ClippedGrads(1.0, 1e-7)):
+        assert is_stand_in(own, 1.0)
+
+
 @pytest.mark.gpu
 def test_gpu_lists_that_cannot_be_clipped_stand_for_the_network_as_before():
     t = torch.ones(3, device='cuda')
