@@ -92,11 +92,14 @@ class ListNorm(torch.Tensor):
 
 
 class ScaledGrads(list, ClippedGrads):
-    """The scaled tensors of a list.  An updater that is given it, as the reference's scripts do, still finds how the network's
-    own gradients are to be clipped."""
+    """The scaled tensors of a list.  An updater works on its network's own gradients alone: given this, as the reference's scripts
+    do, it takes and keeps how those are to be clipped (`own`), by their own norm, and leaves the tensors to the caller."""
     def __init__(self, tensors, max_norm, epsilon):
         list.__init__(self, tensors)
-        ClippedGrads.__init__(self, max_norm, epsilon)
+        self.own = ClippedGrads(max_norm, epsilon)
+
+    max_norm = property(lambda self: self.own.max_norm, lambda self, v: setattr(self.own, 'max_norm', v))
+    epsilon = property(lambda self: self.own.epsilon, lambda self, v: setattr(self.own, 'epsilon', v))
 
 
 def total_norm_constraint(tensor_vars=None, max_norm=0.0, epsilon=1e-7, return_norm=False):
@@ -131,7 +134,7 @@ class OptUpdate(Update):
         self.kind = kind; self.learning_rate = learning_rate
         self.h1, self.h2, self.eps = h1, h2, eps
         self.t_prev = t_prev; self.beta1 = beta1
-        self.clip = grads if isinstance(grads, ClippedGrads) else None
+        self.clip = grads.own if isinstance(grads, ScaledGrads) else grads if isinstance(grads, ClippedGrads) else None
 
     def _lr(self):
         lr = self.learning_rate

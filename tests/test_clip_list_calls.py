@@ -1,5 +1,7 @@
 """updates.total_norm_constraint as a call: what it takes for a list of gradients to clip and what for the network's own, what it
 returns, and what an updater keeps of it."""
+import weakref
+
 import numpy as np
 import pytest
 import torch
@@ -57,6 +59,26 @@ def test_gradients_in_any_iterable_and_parameters_without_one(kind, monkeypatch)
     assert type(updates.total_norm_constraint(kind([on_gpu(1)]), 1.0)) is updates.ScaledGrads
     once = updates.ScaledGrads([on_gpu(1)], 1.0, 1e-7)                  # clipped again
     assert torch.equal(updates.total_norm_constraint(once, 1.0)[0], torch.full((1,), 2.0))
+
+
+def test_an_updater_keeps_no_scaled_tensors():
+    """only how its network's gradients are to be clipped, whatever becomes of the list"""
+    class Net(object):
+        def opt_update(self, kind, lr, h1, h2, eps, max_norm, norm_eps, want_sqrt):
+            self.clipped = max_norm, norm_eps
+    for updater in (updates.adam, updates.sgd, updates.adamax):
+        tensors = [torch.ones(3), torch.ones(2)]
+        gone = weakref.ref(tensors[0])
+        scaled = updates.ScaledGrads(tensors, 5.0, 1e-6)
+        step, _ = updater(scaled, learning_rate=0.1)
+        scaled.max_norm = 4.0                                           # what a script sets later counts, as for the network's own
+        assert step.clip.max_norm == 4.0 and scaled.max_norm == 4.0 and scaled.epsilon == 1e-6
+        del scaled[:]
+        net = Net()
+        step.apply(net)
+        assert net.clipped == (4.0, 1e-6)
+        del tensors, scaled
+        assert gone() is None
 
 
 def test_what_holds_no_gpu_tensor_stands_for_the_network_as_before():
