@@ -7,6 +7,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libasr_amd.so')
+HEADER = os.path.join(os.path.dirname(HERE), 'include', 'asr_amd.h')
 
 
 # Per-file compiler flags.  gemm.hip: hipcc's SLP vectoriser turns the operand split's residual subtractions and the
@@ -40,7 +41,8 @@ def build(force=False, verbose=True, stamps=False):
     srcs = sources()
     if stamps:
         return _build_stamps(srcs)
-    deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')]
+    # the kernels take descriptors from the public header, and the flags of this file
+    deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')] + [HEADER, os.path.abspath(__file__)]
     if not force and os.path.exists(LIB) and all(os.path.getmtime(LIB) >= os.path.getmtime(s) for s in deps):
         return LIB
     objs = []
