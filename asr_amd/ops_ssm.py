@@ -420,17 +420,24 @@ def clip_list(tensors, max_norm, eps=1e-7):
         _fail('tensors: none given')
     if not max_norm >= 0 or not eps >= 0:
         _fail('max_norm %r and eps %r must not be negative' % (max_norm, eps))
-    kinds = [_DTYPES.get(t.dtype) if t.layout is torch.strided else None for t in tensors]
+    kinds = [_DTYPES.get(t.dtype) for t in tensors]
     dev = tensors[0].get_device()
-    for i, t in enumerate(tensors):
-        if kinds[i] is None:
+    if None in kinds or [t.get_device() for t in tensors].count(dev) < len(tensors):
+        for i, t in enumerate(tensors):
             _type('tensors[%d]' % i, t)
-            _fail('tensors[%d]: %s, expected a strided tensor' % (i, t.layout))
-        if t.get_device() != dev:
-            _fail('tensors[%d]: on %s, unlike the others' % (i, t.device))
+            if t.get_device() != dev:
+                _fail('tensors[%d]: on %s, unlike the others' % (i, t.device))
+    try:
+        whole = [t.is_contiguous() for t in tensors]
+    except RuntimeError:                               # compressed sparse layouts have no answer
+        whole = [False]
+    if not all(whole):
+        for i, t in enumerate(tensors):
+            if t.layout is not torch.strided:
+                _fail('tensors[%d]: %s, expected a strided tensor' % (i, t.layout))
     _gpu(dev)
     n, on = len(tensors), tensors[0].device
-    src = [t if t.is_contiguous() else t.contiguous() for t in tensors]
+    src = tensors if all(whole) else [t if c else t.contiguous() for t, c in zip(tensors, whole)]
     sizes = [t.numel() for t in src]
     out, dst = [None] * n, [0] * n
     for dtype, kind in _DTYPES.items():

@@ -34,8 +34,9 @@ def test_lists_that_cannot_be_clipped_stand_for_the_network_as_before():
     for max_norm in (-1.0, np.float32(-2.0)):
         assert is_stand_in([on_gpu(3)], max_norm)
     assert is_stand_in([on_gpu(3)], 1.0, -1e-7)
-    with pytest.raises(ValueError, match='strided'):
-        ops.clip_list([torch.ones(3).to_sparse()], 1.0)
+    for sparse in (torch.eye(3).to_sparse(), torch.eye(3).to_sparse_csr()):
+        with pytest.raises(ValueError, match='strided'):
+            ops.clip_list([torch.ones(3), sparse], 1.0)
 
 
 def clip_on_the_cpu(monkeypatch):
@@ -90,7 +91,7 @@ def test_what_holds_no_gpu_tensor_stands_for_the_network_as_before():
 @pytest.mark.gpu
 def test_gpu_lists_that_cannot_be_clipped_stand_for_the_network_as_before():
     t = torch.ones(3, device='cuda')
-    for bad in ([t.double()], [t, t.long()], [t, torch.ones(2)], [torch.ones(2), t], [t.to_sparse()]):
+    for bad in ([t.double()], [t, t.long()], [t, torch.ones(2)], [torch.ones(2), t], [t.to_sparse()], [torch.eye(3, device='cuda').to_sparse_csr()]):
         assert is_stand_in(bad, 1.0)
     assert is_stand_in([t], -1.0)
 
