@@ -14,8 +14,9 @@ HEADER = os.path.join(os.path.dirname(HERE), 'include', 'asr_amd.h')
 # K-tile joins into v_pk_add_f32 / v_pk_fma_f32, which cost more issue time beside MFMAs than the scalar forms they
 # replace (MI355X_MICROARCH.md, 'price of one filler beside MFMAs'): without it the split GEMMs run 4-6 % faster with
 # bit-identical results (profiles/r03_gemm_no_slp.txt).
-# The state-space layer's files are built without packed fp32 instructions: some of their forms have given wrong results
-# (tests/test_isa_guard.py); the host pass warns that it does not know the feature, which is harmless.
+# The state-space layer's files are built without packed fp32 instructions: builds with some of their forms have shown differing
+# bits, for a reason that is not established (tests/test_isa_guard.py); the host pass warns that it does not know the feature,
+# which is harmless.
 _NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 FILE_FLAGS = {'gemm.hip': ['-fno-slp-vectorize']}
 FILE_FLAGS.update({f: _NO_PACKED_FP32 for f in ('conv.hip', 'sscan_fwd.hip', 'sscan_bwd.hip', 'rmsnorm.hip',

@@ -2,8 +2,8 @@
 //   pre[s,d] = bias[d] + sum_k w[d,k] x[s-(K-1)+k, d],   out = silu(pre) or pre
 // s counts the valid frames of a row in walking order; s < 0 is the carried state.  HBM-bound: one pass over x (and dout).
 // A thread owns V channels and a run of frames and keeps the K-frame window in registers, so a frame is loaded once per run plus
-// the K-1 frames in front of it.  Measured at T 4096, B 16, D 2048, bf16, K 4: forward 117 us (4.6 TB/s of the 0.54 GB it has to
-// move), backward 220 us (3.7 TB/s of 0.81 GB); one f32 frame of 16 x 1024 channels 3.4 us, the launch.
+// the K-1 frames in front of it.  Measured at T 4096, B 16, D 2048, bf16, K 4: forward 113 us (4.8 TB/s of the 0.54 GB it has to
+// move), backward 210 us (3.8 TB/s of 0.81 GB) and 9 for the parts of dw; one f32 frame of 16 x 1024 channels 2.9 us, the launch.
 #include "seq_common.h"
 
 struct ConvArgs {

@@ -4,8 +4,8 @@
 // and can be captured.  HBM-bound for large tensors, launch-bound for small ones: a chunk of CHUNK values of one tensor is a
 // workgroup's work whatever the sizes in the list, three launches in all for up to TENSORS tensors.
 // Squares are summed in double: an f32 square overflows above 1.8e19 and a long f32 sum loses digits.
-// Measured, 56 tensors of 148 MB, f32 and bf16: squares 24 us (6.1 TB/s, part of it from the Infinity Cache), the norm 5, scaling
-// 46 (6.4 TB/s read and written); the host needs 76 us to prepare such a list, beside them.
+// Measured, 56 tensors of 148 MB, f32 and bf16: squares 24 us (6.1 TB/s, part of it from the Infinity Cache), the norm 4, scaling
+// 47 (6.4 TB/s read and written); the host needs 76 us to prepare such a list, beside them.
 #include "seq_common.h"
 
 #define TENSORS 64

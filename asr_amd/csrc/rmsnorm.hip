@@ -4,8 +4,8 @@
 // HBM-bound: a pass reads and writes every tensor once, a row stays in registers between its two uses.  r is rounded to the
 // activation type when it is stored; y is formed from the unrounded sum, and the backward pass forms that sum again from x and
 // the residual (one more read than the stored r would cost, but gradients of what was computed: with the stored r, dw is off by
-// the type's half step).  Measured at 36192 rows x 1024, bf16, with a residual: forward 49 us (6.1 TB/s of the 0.30 GB of its four
-// tensors, some of them still in the Infinity Cache), backward 79 us (4.7 TB/s of 0.37 GB) and 5 for the parts of dw.
+// the type's half step).  Measured at 36192 rows x 1024, bf16, with a residual: forward 48 us (6.2 TB/s of the 0.30 GB of its four
+// tensors, some of them still in the Infinity Cache), backward 77 us (4.8 TB/s of 0.37 GB) and 5 for the parts of dw.
 #include "seq_common.h"
 
 // A row is walked in groups of V columns, a lane to a group.  Where n is no multiple of V the last group is moved back to end with

@@ -4,9 +4,10 @@
 // Tiles are walked from the last to the first.  A tile's states are formed again from the state saved in front of it and kept
 // in registers (16 frames x states, with a), then the adjoint runs back over them.
 //
-// Bound by the vector unit: 14 issue slots per (frame, channel, state) and 4.4 for the sums over lanes, about 110 per (frame,
-// channel).  Measured at T 2048, B 16, D 2048, 16 states, bf16: 855 us, and 31 for the sums over workgroups; those slots are 505 us,
-// the bytes of both passes together 230 us; counters: 81 % of all SIMD cycles issue a vector instruction.
+// Bound by the vector unit: 14 issue slots per (frame, channel, state) and 4.4 for the sums over lanes, 116 per (frame, channel),
+// 410 in all with 16 states.  Measured at T 2048, B 16, D 2048, 16 states, bf16: 866 us, 1.24 times the 700 us of those slots, and 31
+// for the sums over workgroups; the bytes of both passes together are 230 us; counters: 80 % of all SIMD cycles issue a vector
+// instruction.
 #include "sscan.h"
 
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
@@ -45,8 +46,8 @@ __device__ __forceinline__ float sum16(const float (&v)[16], int lane) {
 // Behind a tile's first adjoints, when the first of its states have left their registers, the tile in front of it is called from
 // memory; it goes into the input buffers behind the tile's first barrier, beside the joins.  (Called a tile
 // earlier, as the forward pass does, it costs 30 registers where they are scarcest: one wave per SIMD less, or spills; called
-// half way through the adjoints the spills are 28 registers, and T 2048, B 16, D 2048, bf16 takes 937 us instead of 886; one input
-// buffer instead of two, 840 to 855.)
+// half way through the adjoints the spills are 28 registers, and T 2048, B 16, D 2048, bf16 took 937 us instead of 886; one input
+// buffer instead of two, 850.)
 template <typename TY, int SPL, int NB, bool PRE, bool EDGE>
 __global__ __launch_bounds__(256, 2) void sstate_bwd_kernel(SscanArgs p) {
     constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RS = 8 / SPL;    // RS frames give sixteen sums

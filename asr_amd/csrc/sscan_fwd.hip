@@ -6,10 +6,10 @@
 // One barrier a tile: while a tile's states are walked, the next tile's delta, delta x, B and C go into the other half of the
 // LDS buffers and the tile after that is on its way from memory into registers.
 //
-// Bound by the vector unit: 6 issue slots per (frame, channel, state) (the exponential takes two), about 75 per (frame, channel) for
-// softplus, gate, joins and addresses.  Measured at T 2048, B 16, D 2048, 16 states, bf16: 325 us, 2.0 times the 165 us of those
-// slots at 2.4 GHz on every lane; counters say 80 % of all SIMD cycles issue a vector instruction (at the clock the card holds).
-// One row of T 16384 (24 chunks): 278 us with the pass over chunks.
+// Bound by the vector unit: 6 issue slots per (frame, channel, state) (the exponential takes two) and 59 per (frame, channel) for
+// softplus, gate, joins and addresses, 155 in all with 16 states.  Measured at T 2048, B 16, D 2048, 16 states, bf16: 326 us, 1.24
+// times the 264 us of those slots at 2.4 GHz on every lane; counters say 79 % of all SIMD cycles issue a vector instruction (at the
+// clock the card holds).  One row of T 16384 (24 chunks): 153 us, and 127 for the pass over chunks (slots 135 and 98).
 template <typename TY, int SPL, int NB, bool PRE>
 __global__ __launch_bounds__(256) void sstate_fwd_kernel(SscanArgs p) {
     constexpr int NP = 4 * SPL * NB, TS = SSCAN_TS, RB = (TS * NP + 255) / 256;
@@ -225,11 +225,14 @@ __global__ __launch_bounds__(256) void sscan_step_kernel(SscanArgs p) {
 //     768 / wgs        79   111   129   186   188    as one
 //   backward, one     321   325   326   436   438   441   442   444   687   691   693
 //     chunks          169   239   305   387   435   530   541   547   618   684   753    (2048 / wgs, from 512 on 4)
-// So forward up to 256 as many as make the three workgroups of a CU (at 256 and T 1207, f32, ragged: 168 us with one, 152 with three); backward up to 400 four rounds of the two that a CU holds, which
+// So forward up to 256 as many as make the three workgroups of a CU.  At 256 itself that pays for f32 and for long rows alone
+// (one chunk / three, us, training: T 512 f32 68.4 / 70.5, bf16 68.6 / 70.8; T 1024 142.7 / 132.3, 129.8 / 128.7; T 1207 ragged
+// 165.4 / 150.2, 151.4 / 149.1; T 2262 ragged 309 / 271, 278 / 270).  Backward up to 400 four rounds of the two that a CU holds, which
 // also evens out ragged rows (256 workgroups, T 1207, f32, 4 / 6 / 8 / 10 / 12 chunks: 315 / 308 / 294 / 310 / 309 us), and four chunks
-// where a second round of workgroups would be nearly empty.  (Ragged rows gain less from one chunk: 480 workgroups 417 us, six chunks
-// 386; 544: a step 2 % slower with four.)  A single row (32 workgroups, T 16384): 8 / 16 / 24 / 32 / 64 chunks
+// where a second round of workgroups would be nearly empty.  A single row (32 workgroups, T 16384): 8 / 16 / 24 / 32 / 64 chunks
 // 453 / 310 / 277 / 287 / 286 us.  At least four tiles each.
+// The rule knows the number of workgroups alone, and misses where the rest matters: ragged rows backward (480 workgroups, one chunk
+// 417 us, six 386; 544 workgroups, a step 2 % slower with four than with one), short rows at 256 workgroups (above).
 int sscan_chunks(int T, int B, int D, int G, int backward) {
     const long long wgs = (long long)G * ((D / G + 63) / 64) * B;
     const int nt = sscan_tiles(T);

@@ -420,7 +420,7 @@ int asr_scaling_set_mode(int mode);
  * first.  Buffers written must not overlap any other buffer of the call; workspaces are 16-byte aligned.  All sums run in a
  * fixed order.  Sizes end (ASR_ERR_LIMIT) at B = 65535, D = 2^20, T = 2^21 (convolution) or 2^24 (scan), norm rows below 2^24 and
  * columns up to 2^25, and where a launch would pass 2^32 work items (scan, backward: B T G times twice the states above 4e9;
- * single frames: B D above 2^27).
+ * single frames: B D above 2^27 for the scan, 2^31 for the convolution).
  * ------------------------------------------------------------------------------------------------------------------ */
 
 /* Short causal depthwise convolution over time, 2 <= K <= 8 taps (ASR_ERR_LIMIT above):
