@@ -10,6 +10,7 @@ parameter / gradient buffers, and opt_params_dict exposes the same keys ('t_prev
 `total_norm_constraint` (scripts/dln/ted/exp_prj_lstm_dln.py:17,135-148).  All of them run as the one
 elementwise HIP kernel asr_opt_step; the state tensors are flat, like the parameters.
 """
+import copy
 from collections import OrderedDict
 from collections.abc import Iterable
 
@@ -89,6 +90,12 @@ class ListNorm(torch.Tensor):
     @property
     def value(self):
         return self.item()
+
+    def __reduce_ex__(self, protocol):                 # copied and saved as the plain tensor that it is otherwise
+        return self.as_subclass(torch.Tensor).__reduce_ex__(protocol)
+
+    def __deepcopy__(self, memo):
+        return copy.deepcopy(self.as_subclass(torch.Tensor), memo)
 
 
 class ScaledGrads(list, ClippedGrads):

@@ -1,5 +1,8 @@
 """updates.total_norm_constraint as a call: what it takes for a list of gradients to clip and what for the network's own, what it
 returns, and what an updater keeps of it."""
+import copy
+import io
+import pickle
 import weakref
 
 import numpy as np
@@ -49,6 +52,11 @@ def test_norm_of_a_list_has_a_value_like_the_network_s(monkeypatch):
     assert handle.value is None
     _, norm = updates.total_norm_constraint([on_gpu(3)], 1.0, return_norm=True)
     assert norm.value == 2.5 and norm.shape == (1,) and type(norm.reshape(()) + 1) is torch.Tensor
+    file = io.BytesIO()                                                 # copied and saved like any tensor
+    torch.save(norm, file)
+    file.seek(0)
+    for again in (copy.deepcopy(norm), copy.copy(norm), pickle.loads(pickle.dumps(norm)), torch.load(file, weights_only=True)):
+        assert torch.equal(again, torch.full((1,), 2.5))
 
 
 @pytest.mark.parametrize('kind', [list, tuple, iter, lambda ts: (t for t in ts), lambda ts: dict(enumerate(ts)).values()])
