@@ -9,7 +9,7 @@ are zero and the state is what the last valid frame left.  reverse=True walks ev
 
 Every call is enqueued on the current stream of the tensors' device and allocates its outputs and its workspace through
 torch, so calls on several streams and calls captured into graphs share nothing.  Results do not vary from run to run.
-A wrong argument raises ValueError before anything is launched.
+A wrong argument raises ValueError before anything is launched, a size beyond the C entry's limits (include/asr_amd.h) AsrError.
 """
 import ctypes as C
 import struct
